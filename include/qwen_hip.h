@@ -216,6 +216,81 @@ int qh_add(qh_ctx* ctx, float* d_x, const float* d_delta, int32_t n);
  * of the maximum, NaN never wins unless at index 0. Waits; writes one int to *h_index. */
 int qh_argmax(qh_ctx* ctx, const float* d_v, int32_t n, int32_t* h_index);
 
+/* ------------------------------------------- decoding from a tree of drafts
+ * One forward over several drafted tokens in place of one over a single token (no counterpart in
+ * the reference, whose loop decodes token by token, web/bench.html:121-134). A tree has `nodes`
+ * tokens: node 0 is the last token that was decided, whose K/V row the cache does not hold yet; the
+ * others are drafts, and a node's parent has a lower number. Node i has cache row past + i and rope
+ * position past + its depth. A layer calls qh_rope_append_tree and qh_attention_tree; after the
+ * output head qh_verify_tree walks the tree, and qh_kv_gather moves the accepted rows together, so
+ * that the cache holds past + count positions and the walk's next token becomes the next node 0:
+ *   qh_kv_gather(ctx, &kv, past, &kv, past, layers, kv_heads, head_dim, d_path, nodes, d_count)
+ * All of them are asynchronous and can be captured into a graph from qh_stream. */
+
+/* Host-only: checks the parents (parent[0] = -1, 0 <= parent[i] < i; else QH_ERR_INVALID) and writes
+ * each node's depth [nodes] and the mask of the nodes it sees, itself and its ancestors:
+ * [nodes][ceil(nodes/64)] words, node j at bit j%64 of word j/64. Either output may be NULL. */
+int qh_tree_plan(const int32_t* h_parent, int32_t nodes, int32_t* h_depth, uint64_t* h_mask);
+
+/* qh_rope of q and k at positions past + depth[i] and qh_kv_append of k and v at rows past + i, in
+ * one launch. q [nodes, heads*head_dim], k, v [nodes, kv_heads*head_dim] f32; the rotated q goes to
+ * d_q_out (which may be d_q), the rotated k only into the cache. Depths outside 0 .. nodes-1 are
+ * taken as the nearest of those. past + nodes > capacity or > table_positions is QH_ERR_RANGE. */
+int qh_rope_append_tree(qh_ctx* ctx, const float* d_q, const float* d_k, const float* d_v, const float* d_cos,
+                        const float* d_sin, int32_t table_positions, const int32_t* d_depth, float* d_q_out,
+                        uint16_t* d_key_cache, uint16_t* d_value_cache, int32_t capacity, int32_t heads,
+                        int32_t kv_heads, int32_t head_dim, int32_t past, int32_t nodes);
+
+/* Attention of the tree's queries over the caches of qh_kv_append: node i attends to positions
+ * 0..past-1 and to position past + j for every bit j of its mask row (qh_tree_plan's layout; any
+ * bits are allowed, those from `nodes` on are ignored). A node that sees nothing gets zeros. What a
+ * node does not see has no influence on it, infinities and NaN included. q (rotated), out f32
+ * [nodes, heads*64]; head h reads kv head h / (heads/kv_heads), any group; scale 1/8; head_dim must
+ * be 64; buffers 16-byte aligned. f32 sums (~1e-6 of the output). */
+int qh_attention_tree(qh_ctx* ctx, const float* d_q, const uint16_t* d_key_cache, const uint16_t* d_value_cache,
+                      int32_t capacity, const uint64_t* d_mask, float* d_out, int32_t nodes, int32_t past,
+                      int32_t heads, int32_t kv_heads, int32_t head_dim);
+
+/* Walks the tree from node 0, accepting drafted tokens against the target's probabilities so that
+ * every token is distributed as the target's own sampling would have it (speculative sampling).
+ *   logits [nodes, vocab] f32: row i predicts the token after node i; p_i = softmax(row / temperature)
+ *   draft [nodes, vocab] f32 or NULL: row i holds the probabilities that node i's children were drawn
+ *     from, independently; NULL: the children were not drawn (looked up, or the most likely ones),
+ *     each a distribution of its own with all its weight on its token. Negative values and NaN are 0
+ *   tokens, parent [nodes]; uniform [nodes] f64 in [0, 1)
+ * At a node the children are tested in order: child c, token x, is accepted if uniform[c] * q(x) <
+ * r(x), where r is p at first and max(r - q, 0), normalized, after each rejection. The walk moves to
+ * the first accepted child; where none is, the next token is drawn from r with uniform[0]: the first
+ * index whose running sum of r passes uniform[0] times the total. Temperature 0 is greedy: a child is
+ * accepted if its token is the argmax of its parent's row (qh_argmax's, ties to the lowest index), and
+ * the next token is the argmax; draft and uniform are not read.
+ * Outputs, on the device: path [nodes]: the nodes of the walk in order, node 0 first, then -1; *count
+ * how many they are; *next the token after them. All probabilities and sums are f64. A NaN logit has
+ * probability 0; a row whose largest logit is infinite is uniform over the logits that equal it. A
+ * node whose parent is no earlier node or whose token is outside the vocabulary is never accepted
+ * nor counted as a rejection. Where rejections leave nothing of r, r is p again. */
+int qh_verify_tree(qh_ctx* ctx, const float* d_logits, const float* d_draft, const int32_t* d_tokens,
+                   const int32_t* d_parent, int32_t nodes, int32_t vocab, double temperature,
+                   const double* d_uniform, int32_t* d_path, int32_t* d_count, int32_t* d_next);
+
+/* The f16 caches of one or more layers, in the layout of qh_kv_append: layer i's key cache at d_key +
+ * i*key_stride, its value cache at d_value + i*value_stride (f16 elements; ignored for one layer). */
+typedef struct {
+  uint16_t* d_key;
+  uint16_t* d_value;
+  size_t key_stride, value_stride;
+  int32_t capacity;
+} qh_kv;
+/* Position dst_base + j of dst = position src_base + rows[j] of src, for j < n (and j < *d_count, if
+ * given), every layer and kv head; d_rows NULL: rows[j] = j. Between two caches it copies, forks,
+ * thins or regrows one; within one (src and dst alike) it moves rows together: there an entry whose
+ * source lies before its destination is left as it was, and the others read the rows as they were
+ * before the call. Entries with a row outside the source are left as they were, as are all positions
+ * that no entry names. head_dim a multiple of 8; caches 16-byte aligned with strides that are a
+ * multiple of 8; two caches that overlap without being alike are QH_ERR_INVALID. */
+int qh_kv_gather(qh_ctx* ctx, const qh_kv* src, int32_t src_base, const qh_kv* dst, int32_t dst_base, int32_t layers,
+                 int32_t kv_heads, int32_t head_dim, const int32_t* d_rows, int32_t n, const int32_t* d_count);
+
 /* ------------------------------------------------------------ host helpers
  * The reference quantizer (src/core/quantize.js:36-132), restated for the load path. */
 int qh_quantize_int8(const float* h_w, int32_t rows, int32_t cols, int8_t* h_q,

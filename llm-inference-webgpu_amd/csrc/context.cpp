@@ -575,6 +575,147 @@ int qh_argmax(qh_ctx* ctx, const float* d_v, int32_t n, int32_t* h_index) {
 
 }  // extern "C"
 
+// ------------------------------------------- decoding from a tree of drafts --
+
+// The context's device made current for a launch on its stream, the caller's restored after it.
+namespace {
+struct OnDevice {
+  int before = -1;
+  hipError_t err;
+  explicit OnDevice(int device) {
+    err = hipGetDevice(&before);
+    if (err == hipSuccess && before != device) err = hipSetDevice(device);
+    else before = -1;
+  }
+  ~OnDevice() {
+    if (before >= 0) hipSetDevice(before);
+  }
+};
+}  // namespace
+
+extern "C" {
+
+int qh_rope_append_tree(qh_ctx* ctx, const float* d_q, const float* d_k, const float* d_v, const float* d_cos,
+                        const float* d_sin, int32_t table_positions, const int32_t* d_depth, float* d_q_out,
+                        uint16_t* d_key_cache, uint16_t* d_value_cache, int32_t capacity, int32_t heads,
+                        int32_t kv_heads, int32_t head_dim, int32_t past, int32_t nodes) {
+  QH_CHECK(ctx && d_q && d_k && d_v && d_cos && d_sin && d_depth && d_q_out && d_key_cache && d_value_cache,
+           QH_ERR_INVALID, "rope_append_tree needs q, k, v, the tables, the depths, a q output and both caches");
+  QH_CHECK(nodes >= 1 && past >= 0 && heads >= 1 && kv_heads >= 1 && head_dim >= 2 && head_dim % 2 == 0,
+           QH_ERR_INVALID, "rope_append_tree shape nodes=%d past=%d heads=%d kv_heads=%d head_dim=%d unsupported",
+           nodes, past, heads, kv_heads, head_dim);
+  QH_CHECK((int64_t)heads + 2 * (int64_t)kv_heads <= (1 << 20) / head_dim, QH_ERR_INVALID,
+           "rope_append_tree rows of %d + 2 x %d heads of %d are too wide", heads, kv_heads, head_dim);
+  QH_CHECK((int64_t)past + nodes <= capacity, QH_ERR_RANGE, "cache holds %d of %d; cannot add %d", past, capacity,
+           nodes);
+  QH_CHECK((int64_t)past + nodes <= table_positions, QH_ERR_RANGE, "position %lld exceeds the %d-entry rope table",
+           (long long)past + nodes, table_positions);
+  qh::RopeTreeArgs a{d_q, d_k, d_v, d_cos, d_sin, d_depth, d_q_out, d_key_cache, d_value_cache, capacity,
+                     qh::value_stride(capacity), heads, kv_heads, head_dim, past, nodes};
+  OnDevice on(ctx->device);
+  QH_HIP(on.err);
+  QH_HIP(qh::launch_rope_append_tree(ctx->stream, a));
+  return QH_OK;
+}
+
+int qh_attention_tree(qh_ctx* ctx, const float* d_q, const uint16_t* d_key_cache, const uint16_t* d_value_cache,
+                      int32_t capacity, const uint64_t* d_mask, float* d_out, int32_t nodes, int32_t past,
+                      int32_t heads, int32_t kv_heads, int32_t head_dim) {
+  QH_CHECK(ctx && d_q && d_key_cache && d_value_cache && d_mask && d_out, QH_ERR_INVALID,
+           "attention_tree needs q, both caches, the mask and out");
+  QH_CHECK(head_dim == 64, QH_ERR_INVALID, "attention supports head_dim 64 (got %d)", head_dim);
+  QH_CHECK(kv_heads >= 1 && heads >= kv_heads && heads % kv_heads == 0 && heads <= 65535, QH_ERR_INVALID,
+           "heads %d / kv_heads %d must group evenly, at most 65535 heads", heads, kv_heads);
+  QH_CHECK(nodes >= 1 && past >= 0, QH_ERR_INVALID, "attention_tree needs nodes >= 1 and past >= 0");
+  QH_CHECK((int64_t)past + nodes <= capacity, QH_ERR_RANGE, "attention over %lld positions exceeds capacity %d",
+           (long long)past + nodes, capacity);
+  QH_CHECK((((uintptr_t)d_q | (uintptr_t)d_key_cache | (uintptr_t)d_value_cache | (uintptr_t)d_out) & 15) == 0 &&
+               ((uintptr_t)d_mask & 7) == 0,
+           QH_ERR_INVALID, "q, the caches and out must be 16-byte aligned, the mask 8-byte");
+  qh::TreeAttnArgs a{d_q, d_key_cache, d_value_cache, d_mask, d_out, capacity, qh::value_stride(capacity), heads,
+                     kv_heads, past, nodes};
+  OnDevice on(ctx->device);
+  QH_HIP(on.err);
+  QH_HIP(qh::launch_attention_tree(ctx->stream, a));
+  return QH_OK;
+}
+
+int qh_verify_tree(qh_ctx* ctx, const float* d_logits, const float* d_draft, const int32_t* d_tokens,
+                   const int32_t* d_parent, int32_t nodes, int32_t vocab, double temperature,
+                   const double* d_uniform, int32_t* d_path, int32_t* d_count, int32_t* d_next) {
+  QH_CHECK(ctx && d_logits && d_tokens && d_parent && d_path && d_count && d_next, QH_ERR_INVALID,
+           "verify_tree needs logits, tokens, parents and its three outputs");
+  QH_CHECK(nodes >= 1 && vocab >= 1 && vocab <= 1 << 24, QH_ERR_INVALID,
+           "verify_tree needs nodes >= 1 and a vocabulary of 1..16777216 (nodes %d, vocab %d)", nodes, vocab);
+  QH_CHECK(temperature >= 0.0 && temperature <= 1e30 && (temperature == 0.0 || temperature >= 1e-30), QH_ERR_INVALID,
+           "temperature %g must be 0 or in 1e-30..1e30", temperature);
+  QH_CHECK(temperature == 0.0 || d_uniform, QH_ERR_INVALID, "sampling needs a random number per node");
+  qh::VerifyArgs a{d_logits, temperature == 0.0 ? nullptr : d_draft, d_tokens, d_parent, d_uniform, d_path, d_count,
+                   d_next, temperature, nodes, vocab};
+  OnDevice on(ctx->device);
+  QH_HIP(on.err);
+  QH_HIP(qh::launch_verify_tree(ctx->stream, a));
+  return QH_OK;
+}
+
+}  // extern "C"
+
+// The bytes one layer of a qh_kv spans, and all `layers` of them.
+static size_t kv_span(size_t layer_elements, size_t stride, int32_t layers) {
+  return ((size_t)(layers - 1) * stride + layer_elements) * sizeof(uint16_t);
+}
+
+extern "C" {
+
+int qh_kv_gather(qh_ctx* ctx, const qh_kv* src, int32_t src_base, const qh_kv* dst, int32_t dst_base, int32_t layers,
+                 int32_t kv_heads, int32_t head_dim, const int32_t* d_rows, int32_t n, const int32_t* d_count) {
+  QH_CHECK(ctx && src && dst, QH_ERR_INVALID, "kv_gather needs a context and two caches");
+  QH_CHECK(layers >= 1 && layers <= 65535 && kv_heads >= 1 && kv_heads <= 65535 && head_dim >= 8 &&
+               head_dim % 8 == 0 && head_dim <= 1024,
+           QH_ERR_INVALID, "kv_gather shape layers=%d kv_heads=%d head_dim=%d unsupported (head_dim a multiple of 8)",
+           layers, kv_heads, head_dim);
+  QH_CHECK(n >= 0 && src_base >= 0 && dst_base >= 0 && src->capacity >= 1 && dst->capacity >= 1, QH_ERR_INVALID,
+           "kv_gather needs n, both bases >= 0 and capacities >= 1");
+  const qh_kv* both[2] = {src, dst};
+  size_t kel[2], vel[2];
+  for (int i = 0; i < 2; i++) {
+    const qh_kv* c = both[i];
+    QH_CHECK(c->d_key && c->d_value && (((uintptr_t)c->d_key | (uintptr_t)c->d_value) & 15) == 0, QH_ERR_INVALID,
+             "kv_gather needs 16-byte aligned key and value caches");
+    kel[i] = (size_t)kv_heads * c->capacity * head_dim;
+    vel[i] = qh_value_cache_bytes(c->capacity, kv_heads, head_dim) / 2;
+    QH_CHECK(layers == 1 || (c->key_stride >= kel[i] && c->value_stride >= vel[i] && c->key_stride % 8 == 0 &&
+                             c->value_stride % 8 == 0),
+             QH_ERR_INVALID, "cache strides overlap the caches or break 16-byte alignment");
+  }
+  QH_CHECK((int64_t)dst_base + n <= dst->capacity, QH_ERR_RANGE, "cache holds %d positions; cannot write %d at %d",
+           dst->capacity, n, dst_base);
+  QH_CHECK(src_base <= src->capacity && (d_rows || (int64_t)src_base + n <= src->capacity), QH_ERR_RANGE,
+           "cache holds %d positions; cannot read %d at %d", src->capacity, n, src_base);
+  const bool in_place = src->d_key == dst->d_key && src->d_value == dst->d_value && src->capacity == dst->capacity &&
+                        (layers == 1 || (src->key_stride == dst->key_stride && src->value_stride == dst->value_stride));
+  if (!in_place) {
+    const uintptr_t s0[2] = {(uintptr_t)src->d_key, (uintptr_t)src->d_value};
+    const uintptr_t d0[2] = {(uintptr_t)dst->d_key, (uintptr_t)dst->d_value};
+    const size_t sb[2] = {kv_span(kel[0], src->key_stride, layers), kv_span(vel[0], src->value_stride, layers)};
+    const size_t db[2] = {kv_span(kel[1], dst->key_stride, layers), kv_span(vel[1], dst->value_stride, layers)};
+    for (int i = 0; i < 2; i++)
+      for (int j = 0; j < 2; j++)
+        QH_CHECK(s0[i] + sb[i] <= d0[j] || d0[j] + db[j] <= s0[i], QH_ERR_INVALID,
+                 "the caches overlap without being the same");
+  }
+  if (!n) return QH_OK;
+  qh::GatherArgs a{src->d_key, src->d_value, dst->d_key, dst->d_value, src->key_stride, src->value_stride,
+                   dst->key_stride, dst->value_stride, src->capacity, dst->capacity, src_base, dst_base, layers,
+                   kv_heads, head_dim, n, in_place, d_rows, d_count};
+  OnDevice on(ctx->device);
+  QH_HIP(on.err);
+  QH_HIP(qh::launch_kv_gather(ctx->stream, a));
+  return QH_OK;
+}
+
+}  // extern "C"
+
 extern "C" {
 
 int qh_probe_launch_floor(qh_ctx* ctx, int32_t kind, int32_t blocks, int32_t launches, float* us_per_launch) {

@@ -212,4 +212,23 @@ int qh_synth_tokens(uint64_t seed, const char* name, int32_t vocab, size_t n, in
   return QH_OK;
 }
 
+int qh_tree_plan(const int32_t* h_parent, int32_t nodes, int32_t* h_depth, uint64_t* h_mask) {
+  QH_CHECK(h_parent && nodes >= 1 && (h_depth || h_mask), QH_ERR_INVALID,
+           "tree_plan needs parents, nodes >= 1 and an output");
+  QH_CHECK(h_parent[0] == -1, QH_ERR_INVALID, "node 0 is the root: its parent is -1, not %d", h_parent[0]);
+  for (int32_t i = 1; i < nodes; i++)
+    QH_CHECK(h_parent[i] >= 0 && h_parent[i] < i, QH_ERR_INVALID, "node %d's parent %d is not an earlier node", i,
+             h_parent[i]);
+  const size_t words = ((size_t)nodes + 63) / 64;
+  for (int32_t i = 0; i < nodes; i++) {
+    const int32_t p = h_parent[i];
+    if (h_depth) h_depth[i] = i ? h_depth[p] + 1 : 0;
+    if (!h_mask) continue;
+    uint64_t* row = h_mask + (size_t)i * words;
+    for (size_t w = 0; w < words; w++) row[w] = i ? h_mask[(size_t)p * words + w] : 0;
+    row[i / 64] |= (uint64_t)1 << (i % 64);
+  }
+  return QH_OK;
+}
+
 }  // extern "C"

@@ -223,4 +223,41 @@ size_t argmax_partials_bytes(int n);
 hipError_t launch_nll(hipStream_t s, const float* logits, int vocab, const int32_t* target, int rows, void* partials,
                       double* out);
 size_t nll_partials_bytes(int rows);
+
+// Decoding from a tree of drafted tokens (tree.hip).
+struct RopeTreeArgs {
+  const float *q, *k, *v;    // [nodes][heads | kv_heads | kv_heads][head_dim]
+  const float *cos_t, *sin_t;
+  const int32_t* depth;      // [nodes], taken as 0 .. nodes-1
+  float* q_out;              // may be q
+  uint16_t *kc, *vt;
+  int capacity, vstride, heads, kv_heads, head_dim, past, nodes;
+};
+hipError_t launch_rope_append_tree(hipStream_t s, const RopeTreeArgs& a);
+struct TreeAttnArgs {
+  const float* q;            // [nodes][heads*64], rotated
+  const uint16_t *kc, *vt;
+  const uint64_t* mask;      // [nodes][ceil(nodes / 64)]
+  float* out;                // [nodes][heads*64]
+  int capacity, vstride, heads, kv_heads, past, nodes;
+};
+hipError_t launch_attention_tree(hipStream_t s, const TreeAttnArgs& a);
+struct VerifyArgs {
+  const float *logits, *draft;      // [nodes][vocab]; draft may be null
+  const int32_t *tokens, *parent;   // [nodes]
+  const double* uniform;            // [nodes]; null only at temperature 0
+  int32_t *path, *count, *next;     // [nodes], 1, 1
+  double temperature;
+  int nodes, vocab;
+};
+hipError_t launch_verify_tree(hipStream_t s, const VerifyArgs& a);
+struct GatherArgs {
+  const uint16_t *src_key, *src_value;
+  uint16_t *dst_key, *dst_value;
+  size_t src_key_stride, src_value_stride, dst_key_stride, dst_value_stride;  // f16 elements a layer
+  int src_capacity, dst_capacity, src_base, dst_base, layers, kv_heads, head_dim, n;
+  bool in_place;
+  const int32_t *rows, *count;      // null: 0, 1, 2, ... and n
+};
+hipError_t launch_kv_gather(hipStream_t s, const GatherArgs& a);
 }  // namespace qh

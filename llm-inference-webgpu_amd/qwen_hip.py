@@ -58,6 +58,12 @@ class Weight(ctypes.Structure):
                 ("d_scales", ctypes.c_void_p), ("d_zeros", ctypes.c_void_p)]
 
 
+class KvList(ctypes.Structure):
+    """The f16 caches of one or more layers (qh_kv)."""
+    _fields_ = [("d_key", ctypes.c_void_p), ("d_value", ctypes.c_void_p), ("key_stride", ctypes.c_size_t),
+                ("value_stride", ctypes.c_size_t), ("capacity", ctypes.c_int32)]
+
+
 class Config(ctypes.Structure):
     _fields_ = [("hidden", ctypes.c_int32), ("intermediate", ctypes.c_int32),
                 ("layers", ctypes.c_int32), ("heads", ctypes.c_int32),
@@ -254,6 +260,11 @@ def _declare(lib: ctypes.CDLL) -> None:
         "qh_attention_splitk_list": [vp, vp, vp, vp, sz, sz, i32, i32, vp, i32, i32, i32, i32],
         "qh_attention_list_plan": [i32, i32, i32, vp, vp],
         "qh_argmax": [vp, vp, i32, vp],
+        "qh_tree_plan": [vp, i32, vp, vp],
+        "qh_rope_append_tree": [vp, vp, vp, vp, vp, vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32],
+        "qh_attention_tree": [vp, vp, vp, vp, i32, vp, vp, i32, i32, i32, i32, i32],
+        "qh_verify_tree": [vp, vp, vp, vp, vp, i32, i32, f64, vp, vp, vp, vp],
+        "qh_kv_gather": [vp, vp, i32, vp, i32, i32, i32, i32, vp, i32, vp],
         "qh_quantize_int8": [vp, i32, i32, vp, vp],
         "qh_quantize_int4": [vp, i32, i32, i32, vp, vp, vp],
         "qh_quantize": [vp, i32, vp, i32, i32, i32, i32, vp, vp, vp],
@@ -350,6 +361,17 @@ def quantize_int4(w: np.ndarray, group: int = 128):
     z = np.empty_like(s)
     _check(load_library().qh_quantize_int4(_ptr(w), rows, cols, group, _ptr(q), _ptr(s), _ptr(z)))
     return q, s, z
+
+
+def tree_plan(parent):
+    """(depth int32 [nodes], mask uint64 [nodes, ceil(nodes/64)]) of a tree of drafted tokens given by
+    its parents (parent[0] = -1, every other an earlier node): what rope_append_tree and
+    attention_tree take."""
+    parent = np.ascontiguousarray(parent, np.int32)
+    depth = np.empty(parent.size, np.int32)
+    mask = np.empty((parent.size, (parent.size + 63) // 64), np.uint64)
+    _check(load_library().qh_tree_plan(_ptr(parent), parent.size, _ptr(depth), _ptr(mask)))
+    return depth, mask
 
 
 def rope_tables(head_dim: int, theta: float, positions: int):
@@ -625,6 +647,39 @@ class GpuContext:
         out = ctypes.c_int32()
         _check(self.lib.qh_argmax(self.handle, v.ptr, n, ctypes.byref(out)))
         return out.value
+
+    # Decoding from a tree of drafted tokens (include/qwen_hip.h has the protocol).
+    def rope_append_tree(self, q, k, v, cos, sin, table_positions, depth, q_out, kc, vc, capacity, heads,
+                         kv_heads, head_dim, past, nodes) -> None:
+        """Rotate q (into q_out) and k at positions past + depth[i], and append k and v as rows past + i."""
+        _check(self.lib.qh_rope_append_tree(self.handle, q.ptr, k.ptr, v.ptr, cos.ptr, sin.ptr, table_positions,
+                                            depth.ptr, q_out.ptr, kc.ptr, vc.ptr, capacity, heads, kv_heads,
+                                            head_dim, past, nodes))
+
+    def attention_tree(self, q, kc, vc, capacity, mask, out, nodes, past, heads, kv_heads, head_dim=64) -> None:
+        """Attention of a tree's nodes: each sees positions 0..past-1 and past + j for its mask's bits j."""
+        _check(self.lib.qh_attention_tree(self.handle, q.ptr, kc.ptr, vc.ptr, capacity, mask.ptr, out.ptr, nodes,
+                                          past, heads, kv_heads, head_dim))
+
+    def verify_tree(self, logits, draft, tokens, parent, nodes, vocab, temperature, uniform, path, count,
+                    next_token) -> None:
+        """Walk a tree of drafts, accepting them against the target's logits (`draft`: the draft model's
+        probabilities or None; `uniform`: None only at temperature 0). path, count and next_token are
+        device buffers of int32."""
+        _check(self.lib.qh_verify_tree(self.handle, logits.ptr, draft.ptr if draft else None, tokens.ptr, parent.ptr,
+                                       nodes, vocab, temperature, uniform.ptr if uniform else None, path.ptr,
+                                       count.ptr, next_token.ptr))
+
+    def kv_list(self, key: DeviceBuffer, value: DeviceBuffer, capacity: int, key_stride: int = 0,
+                value_stride: int = 0) -> KvList:
+        """The caches of one or more layers for kv_gather (strides between layers in f16 elements)."""
+        return KvList(key.ptr, value.ptr, key_stride, value_stride, capacity)
+
+    def kv_gather(self, src: KvList, src_base: int, dst: KvList, dst_base: int, layers: int, kv_heads: int,
+                  head_dim: int, rows, n: int, count=None) -> None:
+        """Position dst_base + j of dst = position src_base + rows[j] of src for j < n (j < count[0], if given)."""
+        _check(self.lib.qh_kv_gather(self.handle, ctypes.byref(src), src_base, ctypes.byref(dst), dst_base, layers,
+                                     kv_heads, head_dim, rows.ptr if rows else None, n, count.ptr if count else None))
 
 
 # ------------------------------------------------------------------ model --
