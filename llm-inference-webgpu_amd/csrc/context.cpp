@@ -170,6 +170,7 @@ int qh_close(qh_ctx* ctx) {
   hipSetDevice(ctx->device);
   hipStreamSynchronize(ctx->stream);
   hipFree(ctx->d_scratch);
+  hipFree(ctx->d_tree);
   hipHostFree(ctx->h_pinned);
   hipStreamDestroy(ctx->stream);
   delete ctx;
@@ -591,6 +592,44 @@ struct OnDevice {
     if (before >= 0) hipSetDevice(before);
   }
 };
+
+// Scratch of one call: the context's, which its calls use in order and which grows to what they
+// ask for; or, while the stream is being captured, an allocation of the graph's own, so that
+// graphs may be replayed side by side and outlive the growth.
+struct TreeScratch {
+  qh_ctx* ctx;
+  void* ptr = nullptr;
+  bool own = false;
+  hipError_t err = hipSuccess;
+  TreeScratch(qh_ctx* c, size_t bytes) : ctx(c) {
+    if (!bytes) return;
+    hipStreamCaptureStatus capturing;
+    err = hipStreamIsCapturing(ctx->stream, &capturing);
+    if (err != hipSuccess) return;
+    if (capturing != hipStreamCaptureStatusNone) {
+      err = hipMallocAsync(&ptr, bytes, ctx->stream);
+      own = err == hipSuccess;
+      return;
+    }
+    if (bytes > ctx->tree_bytes) {
+      hipFree(ctx->d_tree);  // waits for the calls that use it
+      ctx->d_tree = nullptr;
+      ctx->tree_bytes = 0;
+      const size_t room = (bytes + bytes / 2 + ((size_t)4 << 20)) & ~(((size_t)1 << 20) - 1);
+      err = hipMalloc(&ctx->d_tree, room);
+      if (err != hipSuccess) {
+        ctx->d_tree = nullptr;
+        hipGetLastError();  // the next call's check is not to find it
+        return;
+      }
+      ctx->tree_bytes = room;
+    }
+    ptr = ctx->d_tree;
+  }
+  ~TreeScratch() {
+    if (own) hipFreeAsync(ptr, ctx->stream);
+  }
+};
 }  // namespace
 
 extern "C" {
@@ -627,6 +666,8 @@ int qh_attention_tree(qh_ctx* ctx, const float* d_q, const uint16_t* d_key_cache
   QH_CHECK(kv_heads >= 1 && heads >= kv_heads && heads % kv_heads == 0 && heads <= 65535, QH_ERR_INVALID,
            "heads %d / kv_heads %d must group evenly, at most 65535 heads", heads, kv_heads);
   QH_CHECK(nodes >= 1 && past >= 0, QH_ERR_INVALID, "attention_tree needs nodes >= 1 and past >= 0");
+  QH_CHECK((int64_t)nodes * heads <= 1 << 22, QH_ERR_INVALID, "attention_tree takes at most 4194304 rows (%d nodes x %d heads)",
+           nodes, heads);
   QH_CHECK((int64_t)past + nodes <= capacity, QH_ERR_RANGE, "attention over %lld positions exceeds capacity %d",
            (long long)past + nodes, capacity);
   QH_CHECK((((uintptr_t)d_q | (uintptr_t)d_key_cache | (uintptr_t)d_value_cache | (uintptr_t)d_out) & 15) == 0 &&
@@ -636,7 +677,11 @@ int qh_attention_tree(qh_ctx* ctx, const float* d_q, const uint16_t* d_key_cache
                      kv_heads, past, nodes};
   OnDevice on(ctx->device);
   QH_HIP(on.err);
-  QH_HIP(qh::launch_attention_tree(ctx->stream, a));
+  const size_t bytes = qh::attention_tree_floats(nodes, past, heads, kv_heads) * sizeof(float);
+  TreeScratch scratch(ctx, bytes);
+  QH_CHECK(scratch.err == hipSuccess, QH_ERR_NOMEM, "attention_tree scratch of %zu bytes: %s", bytes,
+           hipGetErrorString(scratch.err));
+  QH_HIP(qh::launch_attention_tree(ctx->stream, a, static_cast<float*>(scratch.ptr)));
   return QH_OK;
 }
 

@@ -70,6 +70,9 @@ struct qh_ctx {
   size_t scratch_bytes = 0;
   static constexpr size_t kScratchCounterBytes = 16384;
   int32_t* h_pinned = nullptr;  // 4-byte pinned readback slots
+  // Scratch of the tree decoding operators, grown at need (TreeScratch).
+  void* d_tree = nullptr;
+  size_t tree_bytes = 0;
   // This device's copy of the no-allocation entry point's static scratch (or nullptr, and why).
   void* noalloc_scratch = nullptr;
   hipError_t noalloc_err = hipSuccess;
@@ -241,7 +244,9 @@ struct TreeAttnArgs {
   float* out;                // [nodes][heads*64]
   int capacity, vstride, heads, kv_heads, past, nodes;
 };
-hipError_t launch_attention_tree(hipStream_t s, const TreeAttnArgs& a);
+// `part` holds attention_tree_floats floats (no initial contents needed).
+hipError_t launch_attention_tree(hipStream_t s, const TreeAttnArgs& a, float* part);
+size_t attention_tree_floats(int nodes, int past, int heads, int kv_heads);
 struct VerifyArgs {
   const float *logits, *draft;      // [nodes][vocab]; draft may be null
   const int32_t *tokens, *parent;   // [nodes]

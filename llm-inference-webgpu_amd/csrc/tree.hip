@@ -50,68 +50,6 @@ hipError_t launch_rope_append_tree(hipStream_t s, const RopeTreeArgs& a) {
   return hipGetLastError();
 }
 
-// ---------------------------------------------------------------- attention --
-// One block per (node, head): its waves take 64-position chunks in turn, a lane scores one
-// position and owns one output dimension, with an online softmax per wave; the waves' states
-// merge through LDS in wave order.
-__global__ __launch_bounds__(kBlock) void k_attn_tree(TreeAttnArgs a) {
-  constexpr int W = kBlock / kWave;
-  __shared__ float qs[kHeadDim], ps[W][kWave], so[W][kWave], sm[W], sl[W];
-  const int node = blockIdx.x, h = blockIdx.y, g = h / (a.heads / a.kv_heads);
-  const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
-  const size_t row = (size_t)node * a.heads + h;
-  if (threadIdx.x < kHeadDim) qs[threadIdx.x] = a.q[row * kHeadDim + threadIdx.x] * 0.125f;
-  __syncthreads();
-  const uint16_t* kb = a.kc + (size_t)g * a.capacity * kHeadDim;
-  const uint16_t* vb = a.vt + ((size_t)g * kHeadDim + lane) * a.vstride;
-  const uint64_t* mask = a.mask + (size_t)node * ((a.nodes + 63) / 64);
-  const int total = a.past + a.nodes;
-  float m = -INFINITY, l = 0.f, o = 0.f;
-  for (int p0 = w * kWave; p0 < total; p0 += W * kWave) {
-    const int p = p0 + lane, j = p - a.past;
-    const bool see = p < total && (j < 0 || (mask[j >> 6] >> (j & 63) & 1));
-    float s = -INFINITY;
-    if (see) {
-      const uint16_t* kr = kb + (size_t)p * kHeadDim;
-      s = 0.f;
-      for (int d = 0; d < kHeadDim; d++) s = fmaf(qs[d], (float)__builtin_bit_cast(_Float16, kr[d]), s);
-    }
-    uint64_t some = __ballot(see);
-    if (!some) continue;
-    const float mn = fmaxf(m, wave_max(s));
-    const float e = see ? expf(s - mn) : 0.f, alpha = m == -INFINITY ? 0.f : expf(m - mn);
-    l = fmaf(l, alpha, team_sum<64>(e));
-    o *= alpha;
-    m = mn;
-    ps[w][lane] = e;
-    while (some) {
-      const int k = __builtin_ctzll(some);
-      some &= some - 1;
-      o = fmaf(ps[w][k], (float)__builtin_bit_cast(_Float16, vb[p0 + k]), o);
-    }
-  }
-  so[w][lane] = o;
-  if (lane == 0) {
-    sm[w] = m;
-    sl[w] = l;
-  }
-  __syncthreads();
-  if (w) return;
-  float mx = -INFINITY, lt = 0.f, ot = 0.f;
-  for (int v = 0; v < W; v++) mx = fmaxf(mx, sm[v]);
-  for (int v = 0; v < W; v++) {
-    const float wt = sm[v] == -INFINITY ? 0.f : expf(sm[v] - mx);
-    lt = fmaf(sl[v], wt, lt);
-    ot = fmaf(so[v][lane], wt, ot);
-  }
-  a.out[row * kHeadDim + lane] = lt == 0.f ? 0.f : ot / lt;
-}
-
-hipError_t launch_attention_tree(hipStream_t s, const TreeAttnArgs& a) {
-  hipLaunchKernelGGL(k_attn_tree, dim3(a.nodes, a.heads), dim3(kBlock), 0, s, a);
-  return hipGetLastError();
-}
-
 // ------------------------------------------------------------- verification --
 // p = softmax(logits / T) of a node, in f64: p_i = e_i / Z with e_i = exp((l_i - max) / T), a NaN
 // weighing nothing. A node's children are tested in order, x the child's token, q the row of

@@ -73,7 +73,8 @@ def test_attention_tree_refuses(hip, fake):
     for changes, error, what in [({"nodes": 0}, E, "nodes >= 1"), ({"past": -1}, E, "past >= 0"), ({"head_dim": 128}, E, "head_dim 64"),
                                  ({"heads": 5}, E, "group evenly"), ({"kv_heads": 0}, E, "group evenly"),
                                  ({"heads": 1}, E, "group evenly"), ({"past": 16}, R, "exceeds capacity"),
-                                 ({"past": 2**31 - 3}, R, "exceeds capacity"), ({"q": fake.odd}, E, "aligned"),
+                                 ({"past": 2**31 - 3}, R, "exceeds capacity"),
+                                 ({"nodes": 1 << 21, "past": 0, "capacity": 1 << 21}, E, "4194304 rows"), ({"q": fake.odd}, E, "aligned"),
                                  ({"kc": fake.byte}, E, "aligned"), ({"vc": fake.byte}, E, "aligned"), ({"out": fake.odd}, E, "aligned"),
                                  ({"mask": fake.odd}, E, "aligned"), ({"mask": hip.DeviceBuffer(fake, 0, 0)}, E, "the mask")]:
         _refused(hip, "attention_tree", ok, changes, error, what)
