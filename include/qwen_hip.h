@@ -258,7 +258,7 @@ int qh_attention_tree(qh_ctx* ctx, const float* d_q, const uint16_t* d_key_cache
  *   draft [nodes, vocab] f32 or NULL: row i holds the probabilities that node i's children were drawn
  *     from, independently; NULL: the children were not drawn (looked up, or the most likely ones),
  *     each a distribution of its own with all its weight on its token. Negative values and NaN are 0
- *   tokens, parent [nodes]; uniform [nodes] f64 in [0, 1)
+ *   tokens, parent [nodes], at most 1024; uniform [nodes] f64 in [0, 1); vocab at most 2^24
  * At a node the children are tested in order: child c, token x, is accepted if uniform[c] * q(x) <
  * r(x), where r is p at first and max(r - q, 0), normalized, after each rejection. The walk moves to
  * the first accepted child; where none is, the next token is drawn from r with uniform[0]: the first

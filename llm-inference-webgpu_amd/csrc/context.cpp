@@ -690,8 +690,9 @@ int qh_verify_tree(qh_ctx* ctx, const float* d_logits, const float* d_draft, con
                    const double* d_uniform, int32_t* d_path, int32_t* d_count, int32_t* d_next) {
   QH_CHECK(ctx && d_logits && d_tokens && d_parent && d_path && d_count && d_next, QH_ERR_INVALID,
            "verify_tree needs logits, tokens, parents and its three outputs");
-  QH_CHECK(nodes >= 1 && vocab >= 1 && vocab <= 1 << 24, QH_ERR_INVALID,
-           "verify_tree needs nodes >= 1 and a vocabulary of 1..16777216 (nodes %d, vocab %d)", nodes, vocab);
+  QH_CHECK(nodes >= 1 && nodes <= qh::kMaxVerifyNodes && vocab >= 1 && vocab <= qh::kMaxVerifyVocab, QH_ERR_INVALID,
+           "verify_tree takes 1..%d nodes and a vocabulary of 1..%d (nodes %d, vocab %d)", qh::kMaxVerifyNodes,
+           qh::kMaxVerifyVocab, nodes, vocab);
   QH_CHECK(temperature >= 0.0 && temperature <= 1e30 && (temperature == 0.0 || temperature >= 1e-30), QH_ERR_INVALID,
            "temperature %g must be 0 or in 1e-30..1e30", temperature);
   QH_CHECK(temperature == 0.0 || d_uniform, QH_ERR_INVALID, "sampling needs a random number per node");
@@ -699,7 +700,11 @@ int qh_verify_tree(qh_ctx* ctx, const float* d_logits, const float* d_draft, con
                    d_next, temperature, nodes, vocab};
   OnDevice on(ctx->device);
   QH_HIP(on.err);
-  QH_HIP(qh::launch_verify_tree(ctx->stream, a));
+  const size_t bytes = qh::verify_tree_bytes(a);
+  TreeScratch scratch(ctx, bytes);
+  QH_CHECK(scratch.err == hipSuccess, QH_ERR_NOMEM, "verify_tree scratch of %zu bytes: %s", bytes,
+           hipGetErrorString(scratch.err));
+  QH_HIP(qh::launch_verify_tree(ctx->stream, a, scratch.ptr));
   return QH_OK;
 }
 

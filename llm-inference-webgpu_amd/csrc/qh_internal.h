@@ -255,7 +255,10 @@ struct VerifyArgs {
   double temperature;
   int nodes, vocab;
 };
-hipError_t launch_verify_tree(hipStream_t s, const VerifyArgs& a);
+constexpr int kMaxVerifyNodes = 1024, kMaxVerifyVocab = 1 << 24;
+// `scratch` holds verify_tree_bytes bytes (no initial contents needed).
+hipError_t launch_verify_tree(hipStream_t s, const VerifyArgs& a, void* scratch);
+size_t verify_tree_bytes(const VerifyArgs& a);
 struct GatherArgs {
   const uint16_t *src_key, *src_value;
   uint16_t *dst_key, *dst_value;

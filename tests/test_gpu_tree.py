@@ -274,7 +274,7 @@ def _drafts(rng, nodes, vocab, how, width=3, std=2.5):
 
 
 @pytest.mark.parametrize("how", ["greedy", "lookup", "sampled"])
-@pytest.mark.parametrize("nodes,vocab", [(1, 1), (1, 151936), (2, 2), (5, 63), (9, 1000), (33, 257), (6, 4096), (6, 4097), (70, 5000),
+@pytest.mark.parametrize("nodes,vocab", [(1, 1), (1, 151936), (2, 2), (5, 63), (9, 1000), (33, 257), (6, 4096), (6, 4097), (70, 5000), (1024, 130), (3, 300001),
                                          (4, 40961), (12, 151936)])
 def test_verify_tree(ctx, how, nodes, vocab):
     """Path and next token are the walk's, over several draws (f64 on both sides: a pick differs

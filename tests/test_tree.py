@@ -85,7 +85,7 @@ def test_verify_tree_refuses(hip, fake):
     ok = dict(logits=b, draft=None, tokens=b, parent=b, nodes=5, vocab=100, temperature=1.0, uniform=b, path=b, count=b,
               next_token=b)
     E = hip.QwenHipError
-    for changes, error, what in [({"nodes": 0}, E, "nodes >= 1"), ({"vocab": 0}, E, "vocabulary"), ({"vocab": 2**24 + 1}, E, "vocabulary"),
+    for changes, error, what in [({"nodes": 0}, E, "nodes"), ({"nodes": 1025}, E, "1024 nodes"), ({"vocab": 0}, E, "vocabulary"), ({"vocab": 2**24 + 1}, E, "vocabulary"),
                                  ({"temperature": -0.5}, E, "temperature"), ({"temperature": float("nan")}, E, "temperature"),
                                  ({"temperature": float("inf")}, E, "temperature"), ({"temperature": 1e-40}, E, "temperature"),
                                  ({"uniform": None}, E, "random number"),
