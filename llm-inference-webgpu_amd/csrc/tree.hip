@@ -51,50 +51,108 @@ hipError_t launch_rope_append_tree(hipStream_t s, const RopeTreeArgs& a) {
 }
 
 // ------------------------------------------------------------------- gather --
-// grid (1 + head_dim, kv_heads, layers): block x = 0 moves a head's key rows, block 1 + d its row
-// of value dimension d. A block walks its rows upward, a step's reads all before its writes: in
-// place an entry's source is never before its destination (others are skipped), so no step reads
-// what an earlier one wrote.
-__global__ __launch_bounds__(kBlock) void k_kv_gather(GatherArgs a) {
+// Rows of one launch's caches. A block takes a step of key rows (16-byte pieces, kKeyPieces a thread) or of
+// value positions: eight of one dimension's row a thread, gathered by twos of bytes from a run of the
+// source that its neighbours share, and stored as 16 bytes, for kValueDims dimensions a block.
+// In place the blocks of a (layer, head, part) are one, which walks its steps upward, a step's reads
+// all before its writes: an entry's source is never before its destination (others are left), so no
+// step reads what an earlier one wrote. Bound: HBM between two caches; a step's latency in place.
+constexpr int kKeyPieces = 4, kValueDims = 8;
+
+struct GatherCut {
+  int key_blocks, value_blocks;  // along grid x (value_blocks per group of dimensions)
+  int octets;                    // 8-position groups of a value step, a power of two up to kBlock
+};
+
+__device__ __forceinline__ int gather_source(const GatherArgs& a, int n, int j) {  // -1: leave the row
+  if (j < 0 || j >= n) return -1;
+  const int r = a.rows ? a.rows[j] : j;
+  if (r < 0 || r >= a.src_capacity - a.src_base) return -1;
+  return a.in_place && a.src_base + r < a.dst_base + j ? -1 : a.src_base + r;
+}
+
+template <bool IN_PLACE>
+__global__ __launch_bounds__(kBlock) void k_kv_gather(GatherArgs a, GatherCut cut) {
   const int h = blockIdx.y, tid = threadIdx.x;
   const size_t layer = blockIdx.z;
   const int n = a.count ? min(max(*a.count, 0), a.n) : a.n;
-  auto source = [&](int j) -> int {  // the source position of entry j, -1: leave the row
-    if (j >= n) return -1;
-    const int r = a.rows ? a.rows[j] : j;
-    if (r < 0 || r >= a.src_capacity - a.src_base) return -1;
-    return a.in_place && a.src_base + r < a.dst_base + j ? -1 : a.src_base + r;
-  };
-  if (blockIdx.x == 0) {
-    const int vec = a.head_dim / 8, per = max(1, kBlock / vec);  // 16-byte pieces of a row, rows a step
+  if ((int)blockIdx.x < cut.key_blocks) {
+    const int vec = a.head_dim / 8, per = kBlock / vec;  // pieces of a row, rows of a piece's turn
     const v4u* src = reinterpret_cast<const v4u*>(a.src_key + layer * a.src_key_stride) + (size_t)h * a.src_capacity * vec;
     v4u* dst = reinterpret_cast<v4u*>(a.dst_key + layer * a.dst_key_stride) + (size_t)h * a.dst_capacity * vec;
-    for (int j0 = 0; j0 < n; j0 += per) {
-      for (int i0 = 0; i0 < per * vec; i0 += kBlock) {
-        const int i = i0 + tid, j = j0 + i / vec, e = i % vec;
-        const int p = i < per * vec ? source(j) : -1;
-        v4u x{};
-        if (p >= 0) x = src[(size_t)p * vec + e];
-        __syncthreads();
-        if (p >= 0) dst[(size_t)(a.dst_base + j) * vec + e] = x;
-      }
+    const int e = tid % vec, sub = tid / vec;
+    for (int j0 = blockIdx.x * per * kKeyPieces; j0 < n; j0 += per * kKeyPieces) {
+      int p[kKeyPieces];
+      v4u x[kKeyPieces];
+#pragma unroll
+      for (int k = 0; k < kKeyPieces; k++) p[k] = sub < per ? gather_source(a, n, j0 + k * per + sub) : -1;
+#pragma unroll
+      for (int k = 0; k < kKeyPieces; k++)
+        if (p[k] >= 0) x[k] = src[(size_t)p[k] * vec + e];
+      if (IN_PLACE) __syncthreads();
+#pragma unroll
+      for (int k = 0; k < kKeyPieces; k++)
+        if (p[k] >= 0) dst[(size_t)(a.dst_base + j0 + k * per + sub) * vec + e] = x[k];
+      if (!IN_PLACE) return;
     }
     return;
   }
-  const int d = blockIdx.x - 1;
-  const uint16_t* src = a.src_value + layer * a.src_value_stride + ((size_t)h * a.head_dim + d) * value_stride(a.src_capacity);
-  uint16_t* dst = a.dst_value + layer * a.dst_value_stride + ((size_t)h * a.head_dim + d) * value_stride(a.dst_capacity);
-  for (int j0 = 0; j0 < n; j0 += kBlock) {
-    const int j = j0 + tid, p = source(j);
-    uint16_t x = 0;
-    if (p >= 0) x = src[p];
-    __syncthreads();
-    if (p >= 0) dst[a.dst_base + j] = x;
+  const int block = blockIdx.x - cut.key_blocks, group = block / cut.value_blocks;
+  const int at = tid & (cut.octets - 1), turn = kBlock / cut.octets;  // dimensions side by side
+  const int dims = min(kValueDims, a.head_dim - group * kValueDims);
+  const size_t row0 = (size_t)h * a.head_dim + group * kValueDims;
+  const int src_stride = value_stride(a.src_capacity), dst_stride = value_stride(a.dst_capacity);
+  const uint16_t* src = a.src_value + layer * a.src_value_stride + row0 * src_stride;
+  uint16_t* dst = a.dst_value + layer * a.dst_value_stride + row0 * dst_stride;
+  const int first = a.dst_base / 8, octets = (a.dst_base + n + 7) / 8 - first;
+  for (int o0 = block % cut.value_blocks * cut.octets; o0 < octets; o0 += cut.octets) {
+    const int d0 = 8 * (first + o0 + at);  // destination positions d0 .. d0+7
+    int p[8], some = -1, all = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      p[e] = gather_source(a, n, d0 + e - a.dst_base);
+      some = max(some, p[e]);
+      all |= p[e];
+    }
+    uint16_t x[kValueDims][8];
+#pragma unroll
+    for (int k = 0; k < kValueDims; k++) {
+      const int d = tid / cut.octets + k * turn;
+      if (d < dims && some >= 0) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[k][e] = src[(size_t)d * src_stride + max(p[e], 0)];
+      }
+    }
+    if (IN_PLACE) __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kValueDims; k++) {
+      const int d = tid / cut.octets + k * turn;
+      if (d >= dims || some < 0) continue;
+      uint16_t* y = dst + (size_t)d * dst_stride + d0;
+      if (all >= 0) {
+        *reinterpret_cast<v4u*>(y) = v4u{x[k][0] | (uint32_t)x[k][1] << 16, x[k][2] | (uint32_t)x[k][3] << 16,
+                                         x[k][4] | (uint32_t)x[k][5] << 16, x[k][6] | (uint32_t)x[k][7] << 16};
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          if (p[e] >= 0) y[e] = x[k][e];
+      }
+    }
+    if (!IN_PLACE) return;
   }
 }
 
 hipError_t launch_kv_gather(hipStream_t s, const GatherArgs& a) {
-  hipLaunchKernelGGL(k_kv_gather, dim3(1 + a.head_dim, a.kv_heads, a.layers), dim3(kBlock), 0, s, a);
+  GatherCut cut;
+  const int octets = (a.dst_base % 8 + a.n + 7) / 8, groups = (a.head_dim + kValueDims - 1) / kValueDims;
+  cut.octets = kBlock / kValueDims;  // the block's eight dimensions at once, until the row fills it
+  while (cut.octets < octets && cut.octets < kBlock) cut.octets *= 2;
+  const int rows = kBlock / (a.head_dim / 8) * kKeyPieces;
+  cut.key_blocks = a.in_place ? 1 : (a.n + rows - 1) / rows;
+  cut.value_blocks = a.in_place ? 1 : (octets + cut.octets - 1) / cut.octets;
+  const dim3 grid(cut.key_blocks + groups * cut.value_blocks, a.kv_heads, a.layers);
+  if (a.in_place) hipLaunchKernelGGL(k_kv_gather<true>, grid, dim3(kBlock), 0, s, a, cut);
+  else hipLaunchKernelGGL(k_kv_gather<false>, grid, dim3(kBlock), 0, s, a, cut);
   return hipGetLastError();
 }
 
