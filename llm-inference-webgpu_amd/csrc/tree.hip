@@ -57,7 +57,8 @@ hipError_t launch_rope_append_tree(hipStream_t s, const RopeTreeArgs& a) {
 // In place the blocks of a (layer, head, part) are one, which walks its steps upward, a step's reads
 // all before its writes: an entry's source is never before its destination (others are left), so no
 // step reads what an earlier one wrote. Bound: HBM between two caches; a step's latency in place.
-constexpr int kKeyPieces = 4, kValueDims = 8;
+constexpr int kKeyPieces = 4;
+constexpr int kDimsBetween = 4, kDimsInPlace = 8;
 
 struct GatherCut {
   int key_blocks, value_blocks;  // along grid x (value_blocks per group of dimensions)
@@ -65,13 +66,13 @@ struct GatherCut {
 };
 
 __device__ __forceinline__ int gather_source(const GatherArgs& a, int n, int j) {  // -1: leave the row
-  if (j < 0 || j >= n) return -1;
-  const int r = a.rows ? a.rows[j] : j;
-  if (r < 0 || r >= a.src_capacity - a.src_base) return -1;
+  // The row is loaded before the device's count is known.
+  const int r = j >= 0 && j < a.n ? a.rows ? a.rows[j] : j : -1;
+  if (j >= n || r < 0 || r >= a.src_capacity - a.src_base) return -1;
   return a.in_place && a.src_base + r < a.dst_base + j ? -1 : a.src_base + r;
 }
 
-template <bool IN_PLACE>
+template <bool IN_PLACE, int kValueDims>
 __global__ __launch_bounds__(kBlock) void k_kv_gather(GatherArgs a, GatherCut cut) {
   const int h = blockIdx.y, tid = threadIdx.x;
   const size_t layer = blockIdx.z;
@@ -92,7 +93,7 @@ __global__ __launch_bounds__(kBlock) void k_kv_gather(GatherArgs a, GatherCut cu
       if (IN_PLACE) __syncthreads();
 #pragma unroll
       for (int k = 0; k < kKeyPieces; k++)
-        if (p[k] >= 0) dst[(size_t)(a.dst_base + j0 + k * per + sub) * vec + e] = x[k];
+        if (p[k] >= 0) __builtin_nontemporal_store(x[k], &dst[(size_t)(a.dst_base + j0 + k * per + sub) * vec + e]);
       if (!IN_PLACE) return;
     }
     return;
@@ -130,8 +131,8 @@ __global__ __launch_bounds__(kBlock) void k_kv_gather(GatherArgs a, GatherCut cu
       if (d >= dims || some < 0) continue;
       uint16_t* y = dst + (size_t)d * dst_stride + d0;
       if (all >= 0) {
-        *reinterpret_cast<v4u*>(y) = v4u{x[k][0] | (uint32_t)x[k][1] << 16, x[k][2] | (uint32_t)x[k][3] << 16,
-                                         x[k][4] | (uint32_t)x[k][5] << 16, x[k][6] | (uint32_t)x[k][7] << 16};
+        __builtin_nontemporal_store(v4u{x[k][0] | (uint32_t)x[k][1] << 16, x[k][2] | (uint32_t)x[k][3] << 16,
+                                         x[k][4] | (uint32_t)x[k][5] << 16, x[k][6] | (uint32_t)x[k][7] << 16}, reinterpret_cast<v4u*>(y));
       } else {
 #pragma unroll
         for (int e = 0; e < 8; e++)
@@ -144,6 +145,7 @@ __global__ __launch_bounds__(kBlock) void k_kv_gather(GatherArgs a, GatherCut cu
 
 hipError_t launch_kv_gather(hipStream_t s, const GatherArgs& a) {
   GatherCut cut;
+  const int kValueDims = a.in_place ? kDimsInPlace : kDimsBetween;
   const int octets = (a.dst_base % 8 + a.n + 7) / 8, groups = (a.head_dim + kValueDims - 1) / kValueDims;
   cut.octets = kBlock / kValueDims;  // the block's eight dimensions at once, until the row fills it
   while (cut.octets < octets && cut.octets < kBlock) cut.octets *= 2;
@@ -151,8 +153,8 @@ hipError_t launch_kv_gather(hipStream_t s, const GatherArgs& a) {
   cut.key_blocks = a.in_place ? 1 : (a.n + rows - 1) / rows;
   cut.value_blocks = a.in_place ? 1 : (octets + cut.octets - 1) / cut.octets;
   const dim3 grid(cut.key_blocks + groups * cut.value_blocks, a.kv_heads, a.layers);
-  if (a.in_place) hipLaunchKernelGGL(k_kv_gather<true>, grid, dim3(kBlock), 0, s, a, cut);
-  else hipLaunchKernelGGL(k_kv_gather<false>, grid, dim3(kBlock), 0, s, a, cut);
+  if (a.in_place) hipLaunchKernelGGL((k_kv_gather<true, kDimsInPlace>), grid, dim3(kBlock), 0, s, a, cut);
+  else hipLaunchKernelGGL((k_kv_gather<false, kDimsBetween>), grid, dim3(kBlock), 0, s, a, cut);
   return hipGetLastError();
 }
 
