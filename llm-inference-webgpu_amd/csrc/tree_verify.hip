@@ -35,32 +35,65 @@ struct VerifyPart {
   int best;    // the lowest index of `max`; 0x7fffffff: NaN only
 };
 
-// 2^x for x <= 0: 2^rint(x) times the Taylor polynomial of 2^f, |f| <= 1/2 (remainder below 2^-52).
+__device__ __forceinline__ double fma_const(double a, double b, double c) {  // c in scalar registers
+  double r;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
+  return r;
+}
+
+// 2^x for x <= 0 (NaN: 0): 2^rint(x) times 1 + f g(f), f the rest in [-1/2, 1/2] and g the polynomial
+// through (2^f - 1) / f at eleven Chebyshev points (8e-18 off): 11 multiply-adds.
 __device__ __forceinline__ double exp2_f64(double x) {
-  x = fmax(x, -1100.0);  // 2^-1100 is 0
-  const double n = __builtin_rint(x), f = (x - n) * 0.693147180559945309417;
-  double p = 1.0 / 6227020800.0;
-  p = fma(p, f, 1.0 / 479001600.0);
-  p = fma(p, f, 1.0 / 39916800.0);
-  p = fma(p, f, 1.0 / 3628800.0);
-  p = fma(p, f, 1.0 / 362880.0);
-  p = fma(p, f, 1.0 / 40320.0);
-  p = fma(p, f, 1.0 / 5040.0);
-  p = fma(p, f, 1.0 / 720.0);
-  p = fma(p, f, 1.0 / 120.0);
-  p = fma(p, f, 1.0 / 24.0);
-  p = fma(p, f, 1.0 / 6.0);
-  p = fma(p, f, 0.5);
-  p = fma(p, f, 1.0);
+  x = fmax(x, -1100.0);  // 2^-1100 is 0; so is NaN's
+  const double n = __builtin_rint(x), f = x - n;
+  double p = 4.4549605981867755e-10;
+  p = fma_const(p, f, 7.072585949269223e-09);
+  p = fma_const(p, f, 1.0178062445845772e-07);
+  p = fma_const(p, f, 1.321544258792169e-06);
+  p = fma_const(p, f, 1.525273382983612e-05);
+  p = fma_const(p, f, 0.0001540353044173605);
+  p = fma_const(p, f, 0.0013333558146416936);
+  p = fma_const(p, f, 0.009618129107606888);
+  p = fma_const(p, f, 0.0555041086648216);
+  p = fma_const(p, f, 0.24022650695910097);
+  p = fma_const(p, f, 0.6931471805599453);
   p = fma(p, f, 1.0);
   return __builtin_ldexp(p, (int)n);
 }
 
-// e of a logit; k = log2(e) / T.
+// e of a logit l <= m, 0 for NaN; k = log2(e) / T. FINITE: m is.
+template <bool FINITE = false>
 __device__ __forceinline__ double token_weight(float l, float m, double k) {
-  const double d = l == m ? 0.0 : (double)l - (double)m;  // equal infinities weigh 1
-  const double e = exp2_f64(d * k);
-  return l != l ? 0.0 : e;
+  if constexpr (FINITE) return exp2_f64(((double)l - (double)m) * k);
+  return exp2_f64(l == m ? 0.0 : ((double)l - (double)m) * k);  // equal infinities weigh 1
+}
+
+// The maximum over a wave, NaN ignored; every lane gets it.
+template <int CTRL>
+__device__ __forceinline__ float max_step(float v) {
+  return fmaxf(v, dpp32<CTRL>(v));
+}
+__device__ __forceinline__ float verify_max(float v) {
+  v = max_step<kDppMirror>(max_step<kDppHalfMirror>(max_step<kDppQuadXor2>(max_step<kDppQuadXor1>(v))));
+  v = fmaxf(v, swz_xor16(v));
+  return fmaxf(v, __shfl_xor(v, 32));
+}
+
+// Running sums over a wave's lanes: within rows of 16, then the rows before.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double scan_step(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xF, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xF, false);
+  return v + __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ double wave_scan(double v) {
+  v = scan_step<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+  v = scan_step<0x112, 0xF>(v);
+  v = scan_step<0x114, 0xF>(v);
+  v = scan_step<0x118, 0xF>(v);
+  v = scan_step<0x142, 0xA>(v);  // the last lane of a row to the next row
+  return scan_step<0x143, 0xC>(v);  // lane 31 to the upper half
 }
 
 // max(p - a q, 0) from e; a q is 0 for a q that is no probability.
@@ -92,45 +125,62 @@ __device__ __forceinline__ void verify_load(const float* __restrict__ row, int c
 }
 __device__ __forceinline__ bool verify_aligned(const float* row) { return ((uintptr_t)row & 15) == 0; }
 
-// Marks the tokens of `at`'s children that lie in the chunk at c0.
+// What the walk wants of a child: its logit in its parent's row, its draft probability (1 without them).
+struct VerifyKid {
+  float logit, prob;
+};
+
+// The bits 4 g + k of a thread's values (verify_load's, NT threads) that are tokens of `at`'s children; with
+// `kid`, each child's entry is written. Every wave looks for itself: few tokens lie in a chunk.
 template <int NT>
-__device__ __forceinline__ void verify_mark(const VerifyArgs& a, int at, int c0, uint32_t* skip) {
-  for (int i = threadIdx.x; i < kChunkV / 32; i += NT) skip[i] = 0;
-  __syncthreads();
-  for (int i = at + 1 + threadIdx.x; i < a.nodes; i += NT) {
-    const int x = a.tokens[i];
-    if (a.parent[i] == at && x >= c0 && x - c0 < kChunkV) atomicOr(&skip[(x - c0) >> 5], 1u << ((x - c0) & 31));
+__device__ __forceinline__ uint32_t verify_hide(const VerifyArgs& a, int at, int c0, VerifyKid* kid) {
+  const int lane = threadIdx.x & (kWave - 1);
+  uint32_t hide = 0;
+  for (int j0 = at + 1; j0 < a.nodes; j0 += kWave) {
+    const int j = j0 + lane;
+    const bool mine = j < a.nodes && a.parent[j] == at;
+    const int x = mine ? a.tokens[j] : -1;
+    const bool in = x >= c0 && x - c0 < kChunkV && x < a.vocab;
+    uint64_t some = __ballot(in);
+    if (!some) continue;
+    if (kid && in && threadIdx.x < kWave) {
+      const size_t e = (size_t)at * a.vocab + x;
+      kid[j] = {a.logits[e], a.draft ? a.draft[e] : 1.f};
+    }
+    while (some) {
+      const int y = __shfl(x, __builtin_ctzll(some)) - c0;
+      some &= some - 1;
+      if (((y >> 2) & (NT - 1)) == (int)threadIdx.x) hide |= 1u << (4 * (y / (4 * NT)) + (y & 3));
+    }
   }
-  __syncthreads();
+  return hide;
 }
 
-// grid (chunks, nodes). Bound: the logits' bytes (5 TB/s) and the f64 exponentials, about as long.
+// grid (chunks, nodes). Bound: the f64 exponentials (20 f64 operations a logit, 8 cycles each) over the
+// logits' bytes: 64 rows of 151936 take 10.6 us without the exponentials, 13 us from cache alone.
 template <bool GREEDY>
-__global__ __launch_bounds__(kRowsThreads) void k_verify_rows(VerifyArgs a, VerifyPart* __restrict__ part) {
+__global__ __launch_bounds__(kRowsThreads) void k_verify_rows(VerifyArgs a, VerifyPart* __restrict__ part,
+                                                              VerifyKid* __restrict__ kid) {
   constexpr int G = kChunkV / 4 / kRowsThreads, W = kRowsThreads / kWave;
   __shared__ float wm[W];
   __shared__ int wb[W];
   __shared__ double ws[W];
-  __shared__ uint32_t skip[kChunkV / 32];
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
   const int node = blockIdx.y, c0 = blockIdx.x * kChunkV;
   const float* row = a.logits + (size_t)node * a.vocab;
   v4f x[G];
   verify_load<kRowsThreads>(row, c0, a.vocab, verify_aligned(row), NAN, x);
+  uint32_t hide = 0;
+  if constexpr (!GREEDY) {
+    hide = verify_hide<kRowsThreads>(a, node, c0, kid);
+    if (a.draft) hide = 0;
+  }
   float m = -INFINITY;
 #pragma unroll
   for (int g = 0; g < G; g++)
 #pragma unroll
     for (int k = 0; k < 4; k++) m = fmaxf(m, x[g][k]);
-  m = wave_max(m);
-  if (lane == 0) wm[wave] = m;
-  if constexpr (!GREEDY) {
-    if (!a.draft) verify_mark<kRowsThreads>(a, node, c0, skip);
-  }
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < W; w++) m = fmaxf(m, wm[w]);
-  VerifyPart* out = part + (size_t)node * gridDim.x + blockIdx.x;
+  m = verify_max(m);
   if constexpr (GREEDY) {
     int best = 0x7fffffff;
 #pragma unroll
@@ -140,45 +190,75 @@ __global__ __launch_bounds__(kRowsThreads) void k_verify_rows(VerifyArgs a, Veri
         if (x[g][k] == m) best = c0 + 4 * (tid + kRowsThreads * g) + k;
     for (int off = kWave / 2; off > 0; off >>= 1) best = min(best, __shfl_xor(best, off));
     if (lane == 0) wb[wave] = best;
-    __syncthreads();
-    if (tid == 0) {
-#pragma unroll
-      for (int w = 1; w < W; w++) best = min(best, wb[w]);
-      *out = {0.0, m, best};
-    }
   } else {
     const double k2 = 1.44269504088896340736 / a.temperature;
     double s = 0.0;
+    if (fabsf(m) < INFINITY) {
+      if (__any(hide)) {
 #pragma unroll
-    for (int g = 0; g < G; g++)
+        for (int g = 0; g < G; g++)
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        double e = token_weight(x[g][k], m, k2);
-        const int i = 4 * (tid + kRowsThreads * g) + k;
-        if (!a.draft && (skip[i >> 5] >> (i & 31) & 1)) e = 0.0;
-        s += e;
+          for (int k = 0; k < 4; k++) x[g][k] = hide >> (4 * g + k) & 1 ? -INFINITY : x[g][k];
       }
+#pragma unroll
+      for (int g = 0; g < G; g++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) s += token_weight<true>(x[g][k], m, k2);
+    } else {  // equal infinities, or nothing but NaN
+#pragma unroll
+      for (int g = 0; g < G; g++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) s += x[g][k] == m && !(hide >> (4 * g + k) & 1) ? 1.0 : 0.0;
+    }
     s = team_sum<64>(s);
     if (lane == 0) ws[wave] = s;
-    __syncthreads();
-    if (tid == 0) {
+  }
+  if (lane == 0) wm[wave] = m;
+  __syncthreads();
+  if (tid >= W) return;
+  // The waves' maxima and sums to the chunk's.
+  float top = -INFINITY;
 #pragma unroll
-      for (int w = 1; w < W; w++) s += ws[w];
-      *out = {s, m, 0};
-    }
+  for (int w = 0; w < W; w++) top = fmaxf(top, wm[w]);
+  VerifyPart* out = part + (size_t)node * gridDim.x + blockIdx.x;
+  if constexpr (GREEDY) {
+    int best = 0x7fffffff;
+#pragma unroll
+    for (int w = 0; w < W; w++)
+      if (wm[w] == top) best = min(best, wb[w]);
+    if (tid == 0) *out = {0.0, top, best};
+  } else {
+    double s = ws[tid] * token_weight(wm[tid], top, 1.44269504088896340736 / a.temperature);
+#pragma unroll
+    for (int off = 1; off < W; off <<= 1) s += __shfl_xor(s, off);
+    if (tid == 0) *out = {s, top, 0};
   }
 }
 
-// A row's maximum and sum from its chunks' (a wave; every lane gets the same bits).
-__device__ __forceinline__ double verify_row(const VerifyPart* part, int chunks, double k2, float* max) {
+// The maxima and sums of N rows from their chunks' (a wave; every lane gets the same bits, whatever N).
+template <int N>
+__device__ __forceinline__ void verify_row(const VerifyPart* part, int rows, int chunks, double k2, float (&m)[N], double (&s)[N]) {
   const int lane = threadIdx.x & (kWave - 1);
-  float m = -INFINITY;
-  for (int c = lane; c < chunks; c += kWave) m = fmaxf(m, part[c].max);
-  m = wave_max(m);
-  double s = 0.0;
-  for (int c = lane; c < chunks; c += kWave) s = fma(part[c].sum, token_weight(part[c].max, m, k2), s);
-  *max = m;
-  return team_sum<64>(s);
+  VerifyPart p[N];
+#pragma unroll
+  for (int r = 0; r < N; r++) {
+    p[r] = {0.0, -INFINITY, 0};
+    if (r < rows && lane < chunks) p[r] = part[(size_t)r * chunks + lane];
+    m[r] = p[r].max;
+    for (int c = lane + kWave; c < chunks && r < rows; c += kWave) m[r] = fmaxf(m[r], part[(size_t)r * chunks + c].max);
+  }
+#pragma unroll
+  for (int r = 0; r < N; r++) m[r] = verify_max(m[r]);
+#pragma unroll
+  for (int r = 0; r < N; r++) {
+    s[r] = p[r].sum * token_weight(p[r].max, m[r], k2);
+    for (int c = lane + kWave; c < chunks && r < rows; c += kWave) {
+      const VerifyPart q = part[(size_t)r * chunks + c];
+      s[r] = fma(q.sum, token_weight(q.max, m[r], k2), s[r]);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < N; r++) s[r] = team_sum<64>(s[r]);
 }
 
 // The sum of a row's `chunks` residual sums (a wave).
@@ -228,28 +308,39 @@ __global__ __launch_bounds__(kRowsThreads) void k_verify_residual(VerifyArgs a, 
     }
   }
   if (kids <= round) return;
+  // The chunk is on its way while the tests are made; most nodes that have this many children need it.
   const float* row = a.logits + (size_t)node * a.vocab;
   const float* draft = a.draft + (size_t)node * a.vocab;
+  v4f x[G], q[G];
+  verify_load<kRowsThreads>(row, c0, a.vocab, verify_aligned(row), NAN, x);
+  verify_load<kRowsThreads>(draft, c0, a.vocab, verify_aligned(draft), 0.f, q);
   const double k2 = 1.44269504088896340736 / a.temperature;
-  float m;
-  const double inv_z = 1.0 / verify_row(part + (size_t)node * chunks, chunks, k2, &m);
+  float max1[1];
+  double sum1[1];
+  verify_row<1>(part + (size_t)node * chunks, 1, chunks, k2, max1, sum1);
+  const float m = max1[0];
+  const double inv_z = 1.0 / sum1[0];
   VerifyTest t = {0.0, 1.0};
 #pragma unroll
   for (int r = 0; r < kResiduals; r++) {
     if (r > round) break;
-    const int x = a.tokens[kid[r]];
-    if (verify_accept(t, token_weight(row[x], m, k2), inv_z, draft[x], a.uniform[kid[r]])) return;
+    const int token = a.tokens[kid[r]];
+    if (verify_accept(t, token_weight(row[token], m, k2), inv_z, draft[token], a.uniform[kid[r]])) return;
     t.a += t.f;
     if (r < round) verify_reject(t, verify_residual_sum(res + ((size_t)r * a.nodes + node) * chunks, chunks));
   }
-  v4f x[G], q[G];
-  verify_load<kRowsThreads>(row, c0, a.vocab, verify_aligned(row), NAN, x);
-  verify_load<kRowsThreads>(draft, c0, a.vocab, verify_aligned(draft), 0.f, q);
   double s = 0.0;
+  if (fabsf(m) < INFINITY) {
 #pragma unroll
-  for (int g = 0; g < G; g++)
+    for (int g = 0; g < G; g++)
 #pragma unroll
-    for (int k = 0; k < 4; k++) s += residual_weight(token_weight(x[g][k], m, k2), inv_z, t.a, q[g][k]);
+      for (int k = 0; k < 4; k++) s += residual_weight(token_weight<true>(x[g][k], m, k2), inv_z, t.a, q[g][k]);
+  } else {
+#pragma unroll
+    for (int g = 0; g < G; g++)
+#pragma unroll
+      for (int k = 0; k < 4; k++) s += residual_weight(x[g][k] == m ? 1.0 : 0.0, inv_z, t.a, q[g][k]);
+  }
   s = team_sum<64>(s);
   if (lane == 0) ws[wave] = s;
   __syncthreads();
@@ -263,74 +354,88 @@ __global__ __launch_bounds__(kRowsThreads) void k_verify_residual(VerifyArgs a, 
 // One block. Every wave follows the walk by itself over what the other launches left; the block works
 // together on the rows' sums, on further rejections and on the last node's draw.
 __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(VerifyArgs a, const VerifyPart* __restrict__ part,
-                                                              const double* __restrict__ res, int rounds, int chunks) {
+                                                              const VerifyKid* __restrict__ kid, const double* __restrict__ res, int rounds, int chunks) {
   constexpr int G = kChunkV / 4 / kWalkThreads, W = kWalkThreads / kWave;
   static_assert(G == 1, "a thread's share of a chunk is four values in a row");
   static_assert(kMaxVerifyNodes <= kWalkThreads, "a thread a node");
   __shared__ int parent[kMaxVerifyNodes], token[kMaxVerifyNodes], best[kMaxVerifyNodes];
-  __shared__ float row_max[kMaxVerifyNodes], logit[kMaxVerifyNodes], prob[kMaxVerifyNodes];
+  __shared__ float row_max[kMaxVerifyNodes], prob[kMaxVerifyNodes];
   __shared__ double row_sum[kMaxVerifyNodes], uniform[kMaxVerifyNodes], weight[kMaxVerifyNodes];
   __shared__ double red[W], tail[W];
-  __shared__ uint32_t skip[kChunkV / 32];
   __shared__ int wpick[W], wsome[W];
   __shared__ double sums[kMaxVerifyChunks];
+  __shared__ uint8_t accept[kMaxVerifyNodes];
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
   const bool greedy = a.temperature == 0.0, point = !a.draft;
   const double k2 = greedy ? 0.0 : 1.44269504088896340736 / a.temperature;
 
+  VerifyKid own = {0.f, 0.f};
+  int up = -1;
   if (tid < a.nodes) {
     const int p = a.parent[tid], x = a.tokens[tid];
-    const bool ok = verify_candidate(a, tid, p, x);
-    parent[tid] = ok ? p : -1;
-    token[tid] = x;
     if (!greedy) {
       uniform[tid] = a.uniform[tid];
-      if (ok) {
-        logit[tid] = a.logits[(size_t)p * a.vocab + x];
-        prob[tid] = point ? 1.f : a.draft[(size_t)p * a.vocab + x];
-      }
+      own = kid[tid];
     }
+    up = verify_candidate(a, tid, p, x) ? p : -1;
+    parent[tid] = up;
+    token[tid] = x;
+    prob[tid] = own.prob;
   }
-  for (int i = wave; i < a.nodes; i += W) {
-    const VerifyPart* pi = part + (size_t)i * chunks;
-    if (greedy) {
+  if (greedy) {
+    for (int i = wave; i < a.nodes; i += W) {
+      const VerifyPart* pi = part + (size_t)i * chunks;
+      const float l0 = a.logits[(size_t)i * a.vocab];
       float m = -INFINITY;
       int b = 0x7fffffff;
-      for (int c = lane; c < chunks; c += kWave)
-        if (pi[c].max > m || (pi[c].max == m && pi[c].best < b)) {
-          m = pi[c].max;
-          b = pi[c].best;
-        }
-      for (int off = kWave / 2; off > 0; off >>= 1) {
-        const float om = __shfl_xor(m, off);
-        const int ob = __shfl_xor(b, off);
-        if (om > m || (om == m && ob < b)) {
-          m = om;
-          b = ob;
+      for (int c = lane; c < chunks; c += kWave) {
+        const VerifyPart p = pi[c];
+        if (p.max > m || (p.max == m && p.best < b)) {
+          m = p.max;
+          b = p.best;
         }
       }
-      const float l0 = a.logits[(size_t)i * a.vocab];
+      const float top = verify_max(m);
+      b = m == top ? b : 0x7fffffff;
+      for (int off = kWave / 2; off > 0; off >>= 1) b = min(b, __shfl_xor(b, off));
       if (lane == 0) best[i] = l0 != l0 || b == 0x7fffffff ? 0 : b;  // a NaN at index 0 is never beaten
-    } else {
-      float m;
-      const double s = verify_row(pi, chunks, k2, &m);
+    }
+  } else {
+    constexpr int N = 4;
+    for (int i = wave * N; i < a.nodes; i += W * N) {
+      float m[N];
+      double z[N];
+      verify_row<N>(part + (size_t)i * chunks, a.nodes - i, chunks, k2, m, z);
       if (lane == 0) {
-        row_max[i] = m;
-        row_sum[i] = s;
+#pragma unroll
+        for (int r = 0; r < N; r++)
+          if (i + r < a.nodes) {
+            row_max[i + r] = m[r];
+            row_sum[i + r] = z[r];
+          }
       }
     }
   }
   __syncthreads();
-  if (!greedy && tid < a.nodes && parent[tid] >= 0) weight[tid] = token_weight(logit[tid], row_max[parent[tid]], k2);
+  if (!greedy && up >= 0) weight[tid] = own.logit == own.logit ? token_weight(own.logit, row_max[up], k2) : 0.0;
+  // Tests that need no more than the row's sums are made for all nodes at once.
+  bool ok = false;
+  if (greedy && up >= 0) ok = token[tid] == best[up];
   if (point && !greedy) {
-    // A token that an earlier sibling has weighs nothing: it was rejected there.
     __syncthreads();
-    if (tid < a.nodes && parent[tid] >= 0) {
-      bool again = false;
-      for (int j = parent[tid] + 1; j < tid; j++) again |= parent[j] == parent[tid] && token[j] == token[tid];
-      if (again) weight[tid] = 0.0;
+    bool again = false;  // an earlier sibling has the token: it weighs nothing, as it was rejected there
+    if (up >= 0)
+      for (int j = up + 1; j < tid; j++) again |= parent[j] == up && token[j] == token[tid];
+    __syncthreads();
+    if (again) weight[tid] = 0.0;
+    __syncthreads();
+    if (up >= 0) {
+      double rest = 0.0;  // what is left: the other tokens and the children from here on
+      for (int j = a.nodes - 1; j >= tid; j--) rest += parent[j] == up ? weight[j] : 0.0;
+      ok = uniform[tid] * (row_sum[up] + rest) < weight[tid];
     }
   }
+  if (tid < kMaxVerifyNodes) accept[tid] = ok;
   __syncthreads();
 
   // The walk, the same in every thread.
@@ -363,40 +468,35 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(VerifyArgs a, cons
   if (!greedy && !point) inv_z = 1.0 / row_sum[0];
   if (tid == 0) a.path[0] = 0;
   for (int i0 = 1; i0 < a.nodes; i0 += kWave) {
-    // The children of `at` among these 64 nodes; a step down starts over with the new node's.
-    int from = i0;
-    uint64_t some = __ballot(i0 + lane < a.nodes && parent[i0 + lane] == at);
+    // The children of `at` among these 64 nodes; a step down goes on with the new node's.
+    const bool here = i0 + lane < a.nodes;
+    const int over = here ? parent[i0 + lane] : -1;
+    uint64_t some = __ballot(over == at);
+    if (greedy || point) {
+      const uint64_t good = __ballot(here && accept[i0 + lane]);
+      kids |= some != 0;
+      while (some & good) {
+        const int i = __builtin_ctzll(some & good);
+        at = i0 + i;
+        if (tid == 0) a.path[count] = at;
+        count++;
+        some = __ballot(over == at);  // all behind i
+        kids = some != 0;
+      }
+      continue;
+    }
     while (some) {
       const int i = i0 + __builtin_ctzll(some);
       some &= some - 1;
-      if (i < from) continue;
-      bool ok;
-      if (greedy) {
-        ok = token[i] == best[at];
-      } else if (point) {
-        // What is left: the other tokens and the children from here on.
-        double rest = 0.0;
-        for (int j = i + lane; j < a.nodes; j += kWave)
-          if (parent[j] == at) rest += weight[j];
-        rest = row_sum[at] + team_sum<64>(rest);
-        ok = uniform[i] * rest < weight[i];
-      } else {
-        ok = verify_accept(t, weight[i], inv_z, prob[i], uniform[i]);
-      }
-      if (ok) {
+      if (verify_accept(t, weight[i], inv_z, prob[i], uniform[i])) {
         at = i;
         if (tid == 0) a.path[count] = at;
         count++;
-        kids = false;
         tested = 0;
         t = {0.0, 1.0};
-        if (!greedy && !point) inv_z = 1.0 / row_sum[at];
-        from = i + 1;
-        some = __ballot(i0 + lane < a.nodes && parent[i0 + lane] == at);
-        continue;
-      }
-      kids = true;
-      if (!greedy && !point) {
+        inv_z = 1.0 / row_sum[at];
+        some = __ballot(over == at);
+      } else {
         t.a += t.f;
         verify_reject(t, tested < rounds ? verify_residual_sum(res + ((size_t)tested * a.nodes + at) * chunks, chunks)
                                          : residual(t.a));
@@ -422,16 +522,15 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(VerifyArgs a, cons
 
     // A chunk's four weights of a thread.
     auto weigh = [&](int c, double (&w)[4]) {
-      if (without) verify_mark<kWalkThreads>(a, at, c * kChunkV, skip);
       v4f x[G], q[G];
       verify_load<kWalkThreads>(row, c * kChunkV, a.vocab, al, NAN, x);
       if (!plain) verify_load<kWalkThreads>(draft, c * kChunkV, a.vocab, dl, 0.f, q);
+      const uint32_t hide = without ? verify_hide<kWalkThreads>(a, at, c * kChunkV, nullptr) : 0u;
 #pragma unroll
       for (int k = 0; k < 4; k++) {
-        const int i = 4 * tid + k;
         w[k] = token_weight(x[0][k], m, k2);
         if (!plain) w[k] = residual_weight(w[k], inv_z, t.a, q[0][k]);
-        if (without && (skip[i >> 5] >> (i & 31) & 1)) w[k] = 0.0;
+        if (hide >> k & 1) w[k] = 0.0;
       }
     };
     if (again || (!plain && !last)) {  // sums that no launch left
@@ -463,12 +562,7 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(VerifyArgs a, cons
     int c = 0;
     for (int c0 = 0; c0 < chunks; c0 += kWave) {
       const double own = c0 + lane < chunks ? sums[c0 + lane] : 0.0;
-      double s = own;
-      for (int off = 1; off < kWave; off <<= 1) {
-        const double o = __shfl_up(s, off);
-        if (lane >= off) s += o;
-      }
-      s += run;
+      const double s = wave_scan(own) + run;
       const double up = __shfl_up(s, 1), less = lane ? up : run;
       const uint64_t full = __ballot(own > 0.0), hit = __ballot(own > 0.0 && s > target);
       const int pick = hit ? __builtin_ctzll(hit) : full ? 63 - __builtin_clzll(full) : -1;
@@ -482,11 +576,7 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(VerifyArgs a, cons
     double w[4];
     weigh(c, w);
     const double v = w[0] + w[1] + w[2] + w[3];
-    double s = v;
-    for (int off = 1; off < kWave; off <<= 1) {
-      const double o = __shfl_up(s, off);
-      if (lane >= off) s += o;
-    }
+    const double s = wave_scan(v);
     if (lane == kWave - 1) tail[wave] = s;
     __syncthreads();
     double sum = before;
@@ -529,19 +619,21 @@ int verify_chunks(int vocab) { return (vocab + kChunkV - 1) / kChunkV; }
 int verify_rounds(const VerifyArgs& a) { return a.draft ? std::min(kResiduals, a.nodes - 1) : 0; }
 }  // namespace
 
+// Scratch: the chunks' parts, the residuals' sums, the children.
 size_t verify_tree_bytes(const VerifyArgs& a) {
-  return (size_t)a.nodes * verify_chunks(a.vocab) * (sizeof(VerifyPart) + verify_rounds(a) * sizeof(double));
+  return (size_t)a.nodes * (verify_chunks(a.vocab) * (sizeof(VerifyPart) + verify_rounds(a) * sizeof(double)) + sizeof(VerifyKid));
 }
 
 hipError_t launch_verify_tree(hipStream_t s, const VerifyArgs& a, void* scratch) {
   const int chunks = verify_chunks(a.vocab), rounds = verify_rounds(a);
   VerifyPart* part = static_cast<VerifyPart*>(scratch);
   double* res = reinterpret_cast<double*>(part + (size_t)a.nodes * chunks);
+  VerifyKid* kid = reinterpret_cast<VerifyKid*>(res + (size_t)rounds * a.nodes * chunks);
   const dim3 grid(chunks, a.nodes), block(kRowsThreads);
-  if (a.temperature == 0.0) hipLaunchKernelGGL(k_verify_rows<true>, grid, block, 0, s, a, part);
-  else hipLaunchKernelGGL(k_verify_rows<false>, grid, block, 0, s, a, part);
+  if (a.temperature == 0.0) hipLaunchKernelGGL(k_verify_rows<true>, grid, block, 0, s, a, part, kid);
+  else hipLaunchKernelGGL(k_verify_rows<false>, grid, block, 0, s, a, part, kid);
   for (int r = 0; r < rounds; r++) hipLaunchKernelGGL(k_verify_residual, grid, block, 0, s, a, part, res, r);
-  hipLaunchKernelGGL(k_verify_walk, dim3(1), dim3(kWalkThreads), 0, s, a, part, res, rounds, chunks);
+  hipLaunchKernelGGL(k_verify_walk, dim3(1), dim3(kWalkThreads), 0, s, a, part, kid, res, rounds, chunks);
   return hipGetLastError();
 }
 
