@@ -15,8 +15,8 @@
 // those borders by more than the probabilities between them.
 //
 // Launches: every row's chunks of kChunkV logits on blocks of their own (k_verify_rows: maximum, sum,
-// argmax); with draft probabilities, F after the first and after the second rejection of every node
-// that has them (k_verify_residual); then one block walks the tree over what those left
+// argmax); with draft probabilities, F after the first, second and third rejection of every node that
+// comes to them (k_verify_residual); then one block walks the tree over what those left
 // (k_verify_walk), reading one chunk again to find the token.
 #include <algorithm>
 
@@ -27,7 +27,7 @@ namespace qh {
 constexpr int kChunkV = 4096;
 constexpr int kMaxVerifyChunks = kMaxVerifyVocab / kChunkV;
 constexpr int kRowsThreads = 256, kWalkThreads = 1024;
-constexpr int kResiduals = 2;  // rejections of a node whose F has launches of its own
+constexpr int kResiduals = 3;  // rejections of a node whose F has a launch of its own
 
 struct VerifyPart {
   double sum;  // of e relative to `max`, without the children's tokens where there are no draft probabilities
@@ -235,15 +235,23 @@ __global__ __launch_bounds__(kRowsThreads) void k_verify_rows(VerifyArgs a, Veri
   }
 }
 
-// The maxima and sums of N rows from their chunks' (a wave; every lane gets the same bits, whatever N).
+// The maxima and sums of N rows from their chunks' (a wave; every lane gets the same bits, whatever N):
+// the first 64 chunks of each are loaded by verify_parts, which the caller may do long before.
 template <int N>
-__device__ __forceinline__ void verify_row(const VerifyPart* part, int rows, int chunks, double k2, float (&m)[N], double (&s)[N]) {
+__device__ __forceinline__ void verify_parts(const VerifyPart* part, int rows, int chunks, VerifyPart (&p)[N]) {
   const int lane = threadIdx.x & (kWave - 1);
-  VerifyPart p[N];
 #pragma unroll
   for (int r = 0; r < N; r++) {
-    p[r] = {0.0, -INFINITY, 0};
+    p[r] = {0.0, -INFINITY, 0x7fffffff};
     if (r < rows && lane < chunks) p[r] = part[(size_t)r * chunks + lane];
+  }
+}
+template <int N>
+__device__ __forceinline__ void verify_row(const VerifyPart* part, const VerifyPart (&p)[N], int rows, int chunks, double k2,
+                                           float (&m)[N], double (&s)[N]) {
+  const int lane = threadIdx.x & (kWave - 1);
+#pragma unroll
+  for (int r = 0; r < N; r++) {
     m[r] = p[r].max;
     for (int c = lane + kWave; c < chunks && r < rows; c += kWave) m[r] = fmaxf(m[r], part[(size_t)r * chunks + c].max);
   }
@@ -288,6 +296,7 @@ __device__ __forceinline__ bool verify_accept(const VerifyTest& t, double e, dou
 // grid (chunks, nodes), for round = 0, 1, ...: the chunk's part of F after a node's first round + 1
 // children were rejected, if they were (res [round][node][chunk]).
 __global__ __launch_bounds__(kRowsThreads) void k_verify_residual(VerifyArgs a, const VerifyPart* __restrict__ part,
+                                                                  const VerifyKid* __restrict__ kids_of,
                                                                   double* __restrict__ res, int round) {
   constexpr int G = kChunkV / 4 / kRowsThreads, W = kRowsThreads / kWave;
   __shared__ double ws[W];
@@ -317,15 +326,17 @@ __global__ __launch_bounds__(kRowsThreads) void k_verify_residual(VerifyArgs a, 
   const double k2 = 1.44269504088896340736 / a.temperature;
   float max1[1];
   double sum1[1];
-  verify_row<1>(part + (size_t)node * chunks, 1, chunks, k2, max1, sum1);
+  VerifyPart p[1];
+  verify_parts<1>(part + (size_t)node * chunks, 1, chunks, p);
+  verify_row<1>(part + (size_t)node * chunks, p, 1, chunks, k2, max1, sum1);
   const float m = max1[0];
   const double inv_z = 1.0 / sum1[0];
   VerifyTest t = {0.0, 1.0};
 #pragma unroll
   for (int r = 0; r < kResiduals; r++) {
     if (r > round) break;
-    const int token = a.tokens[kid[r]];
-    if (verify_accept(t, token_weight(row[token], m, k2), inv_z, draft[token], a.uniform[kid[r]])) return;
+    const VerifyKid c = kids_of[kid[r]];
+    if (verify_accept(t, token_weight(c.logit, m, k2), inv_z, c.prob, a.uniform[kid[r]])) return;
     t.a += t.f;
     if (r < round) verify_reject(t, verify_residual_sum(res + ((size_t)r * a.nodes + node) * chunks, chunks));
   }
@@ -351,265 +362,328 @@ __global__ __launch_bounds__(kRowsThreads) void k_verify_residual(VerifyArgs a, 
   }
 }
 
-// One block. Every wave follows the walk by itself over what the other launches left; the block works
-// together on the rows' sums, on further rejections and on the last node's draw.
+__device__ __forceinline__ double lane_value(double v, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane);
+  const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// One block over what the other launches left: the rows' maxima and sums, the walk, the last node's draw.
+// Bound: latency (three rounds of loads, one after another, and the f64 arithmetic between them).
 __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(VerifyArgs a, const VerifyPart* __restrict__ part,
-                                                              const VerifyKid* __restrict__ kid, const double* __restrict__ res, int rounds, int chunks) {
-  constexpr int G = kChunkV / 4 / kWalkThreads, W = kWalkThreads / kWave;
-  static_assert(G == 1, "a thread's share of a chunk is four values in a row");
+                                                              const VerifyKid* __restrict__ kid,
+                                                              const double* __restrict__ res, int rounds, int chunks) {
+  constexpr int W = kWalkThreads / kWave, N = 4;  // N rows at once to a wave
+  static_assert(kChunkV == 4 * kWalkThreads, "a thread's share of a chunk is four values in a row");
   static_assert(kMaxVerifyNodes <= kWalkThreads, "a thread a node");
-  __shared__ int parent[kMaxVerifyNodes], token[kMaxVerifyNodes], best[kMaxVerifyNodes];
+  __shared__ int parent[kMaxVerifyNodes], token[kMaxVerifyNodes];
   __shared__ float row_max[kMaxVerifyNodes], prob[kMaxVerifyNodes];
   __shared__ double row_sum[kMaxVerifyNodes], uniform[kMaxVerifyNodes], weight[kMaxVerifyNodes];
-  __shared__ double red[W], tail[W];
-  __shared__ int wpick[W], wsome[W];
+  __shared__ double red[W];
   __shared__ double sums[kMaxVerifyChunks];
-  __shared__ uint8_t accept[kMaxVerifyNodes];
+  __shared__ uint16_t list[kMaxVerifyNodes];
+  __shared__ int walked[3], wpick[W], wsome[W];
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-  const bool greedy = a.temperature == 0.0, point = !a.draft;
-  const double k2 = greedy ? 0.0 : 1.44269504088896340736 / a.temperature;
+  const bool point = !a.draft;
+  const double k2 = 1.44269504088896340736 / a.temperature;
 
+  VerifyPart first[N];
+  verify_parts<N>(part + (size_t)wave * N * chunks, a.nodes - wave * N, chunks, first);
   VerifyKid own = {0.f, 0.f};
   int up = -1;
   if (tid < a.nodes) {
     const int p = a.parent[tid], x = a.tokens[tid];
-    if (!greedy) {
-      uniform[tid] = a.uniform[tid];
-      own = kid[tid];
-    }
+    uniform[tid] = a.uniform[tid];
+    own = kid[tid];
     up = verify_candidate(a, tid, p, x) ? p : -1;
     parent[tid] = up;
     token[tid] = x;
     prob[tid] = own.prob;
   }
-  if (greedy) {
-    for (int i = wave; i < a.nodes; i += W) {
-      const VerifyPart* pi = part + (size_t)i * chunks;
-      const float l0 = a.logits[(size_t)i * a.vocab];
-      float m = -INFINITY;
-      int b = 0x7fffffff;
-      for (int c = lane; c < chunks; c += kWave) {
-        const VerifyPart p = pi[c];
+  for (int i = wave * N; i < a.nodes; i += W * N) {
+    const VerifyPart* pi = part + (size_t)i * chunks;
+    if (i != wave * N) verify_parts<N>(pi, a.nodes - i, chunks, first);
+    float m[N];
+    double z[N];
+    verify_row<N>(pi, first, a.nodes - i, chunks, k2, m, z);
+    if (lane == 0) {
+#pragma unroll
+      for (int r = 0; r < N; r++)
+        if (i + r < a.nodes) {
+          row_max[i + r] = m[r];
+          row_sum[i + r] = z[r];
+        }
+    }
+  }
+  __syncthreads();
+  if (up >= 0) weight[tid] = token_weight(own.logit, row_max[up], k2);
+  __syncthreads();
+
+  int at = 0, count = 1;
+  bool kids = false;          // `at` has children, all of them rejected
+  VerifyTest t = {0.0, 1.0};  // with draft probabilities: how far the tests of `at` have come,
+  int tested = 0;             // after so many rejections
+  double inv_z = 1.0 / row_sum[0];
+  // The chunks' sums over the row of `at` where no launch left them, a chunk to a wave: of max(p - t.a q, 0)
+  // or, with t.a = 0, of e. On one CU the f64 arithmetic takes about 50 us for 151936 tokens.
+  auto make_sums = [&]() {
+    const float* row = a.logits + (size_t)at * a.vocab;
+    const float* draft = t.a == 0.0 ? nullptr : a.draft + (size_t)at * a.vocab;
+    __syncthreads();
+    for (int c = wave; c < chunks; c += W) {
+      double s = 0.0;
+      for (int i = c * kChunkV + lane; i < min(a.vocab, (c + 1) * kChunkV); i += kWave) {
+        const double e = token_weight(row[i], row_max[at], k2);
+        s += draft ? residual_weight(e, inv_z, t.a, draft[i]) : e;
+      }
+      s = team_sum<64>(s);
+      if (lane == 0) sums[c] = s;
+    }
+    __syncthreads();
+  };
+  if (tid == 0) a.path[0] = 0;
+  if (point) {
+    // The first wave walks: a node's children to its lanes, tested all at once.
+    if (wave == 0) {
+      for (;;) {
+        int n = 0;
+        for (int j0 = at + 1; j0 < a.nodes; j0 += kWave) {
+          const bool mine = j0 + lane < a.nodes && parent[j0 + lane] == at;
+          const uint64_t b = __ballot(mine);
+          if (mine) list[n + __builtin_popcountll(b & (((uint64_t)1 << lane) - 1))] = (uint16_t)(j0 + lane);
+          n += __builtin_popcountll(b);
+        }
+        kids = n > 0;
+        if (!n) break;
+        wave_lds_handoff();
+        // A token that an earlier child has weighs nothing: it was rejected there.
+        for (int b0 = 0; b0 < n; b0 += kWave) {
+          const int i = b0 + lane < n ? list[b0 + lane] : 0, x = b0 + lane < n ? token[i] : -1;
+          bool again = false;
+          for (int c = 0; c < b0; c++) again |= token[list[c]] == x;
+          for (int c = 0; c < min(kWave, n - b0); c++) again |= lane > c && __builtin_amdgcn_readlane(x, c) == x;
+          if (again && x >= 0) weight[i] = 0.0;
+        }
+        wave_lds_handoff();
+        // What is left at a child: the tokens that are none, and the children from it on.
+        double left = row_sum[at];
+        int to = -1;
+        for (int b0 = (n - 1) & ~(kWave - 1); b0 >= 0; b0 -= kWave) {
+          const int i = b0 + lane < n ? list[b0 + lane] : 0;
+          const double w = b0 + lane < n ? weight[i] : 0.0;
+          double rest = 0.0;
+          for (int c = min(kWave, n - b0) - 1; c >= 0; c--) {
+            left += lane_value(w, c);
+            if (lane == c) rest = left;
+          }
+          const uint64_t good = __ballot(b0 + lane < n && uniform[i] * rest < w);
+          if (good) to = list[b0 + __builtin_ctzll(good)];
+        }
+        if (to < 0) break;
+        at = to;
+        if (lane == 0) a.path[count] = at;
+        count++;
+        wave_lds_handoff();
+      }
+      if (lane == 0) {
+        walked[0] = at;
+        walked[1] = count;
+        walked[2] = kids;
+      }
+    }
+    __syncthreads();
+    at = walked[0];
+    count = walked[1];
+    kids = walked[2];
+  } else {
+    // Every wave walks for itself, with the same bits, and they meet in make_sums.
+    for (int i0 = 1; i0 < a.nodes; i0 += kWave) {
+      const int over = i0 + lane < a.nodes ? parent[i0 + lane] : -1;
+      uint64_t some = __ballot(over == at);
+      while (some) {
+        const int i = i0 + __builtin_ctzll(some);
+        some &= some - 1;
+        if (verify_accept(t, weight[i], inv_z, prob[i], uniform[i])) {
+          at = i;
+          if (tid == 0) a.path[count] = at;
+          count++;
+          tested = 0;
+          t = {0.0, 1.0};
+          inv_z = 1.0 / row_sum[at];
+          some = __ballot(over == at);  // all behind the step
+        } else {
+          t.a += t.f;
+          if (tested >= rounds) make_sums();
+          verify_reject(t, verify_residual_sum(tested < rounds ? res + ((size_t)tested * a.nodes + at) * chunks : sums, chunks));
+          tested++;
+        }
+      }
+    }
+  }
+
+  int next = 0;
+  // The weights that are left at the last node: the residual's, or e, without the children's tokens
+  // where they are points (all of them again if nothing else is left).
+  const VerifyPart* pa = part + (size_t)at * chunks;
+  const float m = row_max[at];
+  const bool plain = point || t.a == 0.0;
+  const bool without = point && kids && row_sum[at] != 0.0;
+  const double* last = !plain && tested <= rounds ? res + ((size_t)(tested - 1) * a.nodes + at) * chunks : nullptr;
+  const bool no_sums = plain ? point && kids && !without : !last;  // no launch left the chunks' sums
+  const float* row = a.logits + (size_t)at * a.vocab;
+  const float* draft = plain ? nullptr : a.draft + (size_t)at * a.vocab;
+  const bool al = verify_aligned(row), dl = verify_aligned(draft);
+
+  // A chunk's four weights of a thread.
+  auto weigh = [&](int c, double (&w)[4]) {
+    v4f x[1], q[1];
+    verify_load<kWalkThreads>(row, c * kChunkV, a.vocab, al, NAN, x);
+    if (!plain) verify_load<kWalkThreads>(draft, c * kChunkV, a.vocab, dl, 0.f, q);
+    uint32_t hide = 0;
+    if (without)
+      for (int i0 = at + 1; i0 < a.nodes; i0 += kWave) {
+        const int i = i0 + lane, x0 = i < a.nodes && parent[i] == at ? token[i] - c * kChunkV : -1;
+        uint64_t some = __ballot(x0 >= 0 && x0 < kChunkV);
+        while (some) {
+          const int y = __builtin_amdgcn_readlane(x0, __builtin_ctzll(some));
+          some &= some - 1;
+          if (y >> 2 == tid) hide |= 1u << (y & 3);
+        }
+      }
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      w[k] = token_weight(x[0][k], m, k2);
+      if (!plain) w[k] = residual_weight(w[k], inv_z, t.a, q[0][k]);
+      if (hide >> k & 1) w[k] = 0.0;
+    }
+  };
+  if (no_sums && plain) make_sums();  // a residual's are there from the last rejection
+  auto chunk_sum = [&](int c) -> double {
+    return c >= chunks ? 0.0 : no_sums ? sums[c] : plain ? pa[c].sum * token_weight(pa[c].max, m, k2) : last[c];
+  };
+  // The first chunk whose running sum passes the target (every wave for itself, 64 chunks at a time);
+  // where the rounding of the total leaves none, the last one with a weight.
+  double u = uniform[0];
+  u = u > 0.0 ? u : 0.0;
+  if (u >= 1.0) u = 1.0 - 0x1p-53;
+  const double sum0 = chunk_sum(lane), scan0 = wave_scan(sum0);
+  double total = lane_value(scan0, kWave - 1);
+  for (int c0 = kWave; c0 < chunks; c0 += kWave) total += lane_value(wave_scan(chunk_sum(c0 + lane)), kWave - 1);
+  const double target = u * total;
+  double before = 0.0, run = 0.0;
+  int c = 0;
+  for (int c0 = 0; c0 < chunks; c0 += kWave) {
+    const double mine = c0 ? chunk_sum(c0 + lane) : sum0;
+    const double s = (c0 ? wave_scan(mine) : scan0) + run;
+    const uint64_t full = __ballot(mine > 0.0), hit = __ballot(mine > 0.0 && s > target);
+    const int pick = hit ? __builtin_ctzll(hit) : full ? 63 - __builtin_clzll(full) : -1;
+    if (pick >= 0) {
+      c = c0 + pick;
+      before = pick ? lane_value(s, pick - 1) : run;
+    }
+    if (hit) break;
+    run = lane_value(s, kWave - 1);
+  }
+  double w[4];
+  weigh(c, w);
+  const double s = wave_scan(w[0] + w[1] + w[2] + w[3]);
+  __syncthreads();
+  if (lane == kWave - 1) red[wave] = s;
+  __syncthreads();
+  double sum = before;
+#pragma unroll
+  for (int k = 0; k < W; k++) sum += k < wave ? red[k] : 0.0;
+  sum += s - (w[0] + w[1] + w[2] + w[3]);
+  int pick = -1, some = -1;
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    sum += w[k];
+    if (w[k] > 0.0) {
+      some = c * kChunkV + 4 * tid + k;
+      if (sum > target && pick < 0) pick = some;
+    }
+  }
+  const uint64_t hits = __ballot(pick >= 0), full = __ballot(some >= 0);
+  pick = hits ? __builtin_amdgcn_readlane(pick, __builtin_ctzll(hits)) : -1;
+  some = full ? __builtin_amdgcn_readlane(some, 63 - __builtin_clzll(full)) : -1;
+  if (lane == 0) {
+    wpick[wave] = pick;
+    wsome[wave] = some;
+  }
+  __syncthreads();
+  if (wave == 0) {
+    pick = lane < W ? wpick[lane] : -1;
+    some = lane < W ? wsome[lane] : -1;
+    const uint64_t wh = __ballot(pick >= 0), wf = __ballot(some >= 0);
+    // Behind the chunk's own rounding: its last token with a weight; 0 where no token has one.
+    next = wh ? __builtin_amdgcn_readlane(pick, __builtin_ctzll(wh))
+              : wf ? __builtin_amdgcn_readlane(some, 63 - __builtin_clzll(wf)) : 0;
+  }
+  if (tid == 0) {
+    *a.count = count;
+    *a.next = next;
+  }
+  if (tid >= count && tid < a.nodes) a.path[tid] = -1;
+}
+
+// Temperature 0: the rows' argmaxima, four rows at once to a wave, then the walk. At least `nodes` threads.
+__global__ __launch_bounds__(kWalkThreads) void k_verify_walk_greedy(VerifyArgs a, const VerifyPart* __restrict__ part, int chunks) {
+  constexpr int N = 4;
+  __shared__ int parent[kMaxVerifyNodes], token[kMaxVerifyNodes], best[kMaxVerifyNodes];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, waves = blockDim.x / kWave;
+  if (tid < a.nodes) {
+    const int p = a.parent[tid], x = a.tokens[tid];
+    parent[tid] = verify_candidate(a, tid, p, x) ? p : -1;
+    token[tid] = x;
+  }
+  for (int i = wave * N; i < a.nodes; i += waves * N) {
+    const VerifyPart* pi = part + (size_t)i * chunks;
+    VerifyPart first[N];
+    float l0[N];
+    verify_parts<N>(pi, a.nodes - i, chunks, first);
+#pragma unroll
+    for (int r = 0; r < N; r++) l0[r] = a.logits[(size_t)min(i + r, a.nodes - 1) * a.vocab];
+#pragma unroll
+    for (int r = 0; r < N; r++) {
+      float m = first[r].max;
+      int b = first[r].best;
+      for (int c = lane + kWave; c < chunks && i + r < a.nodes; c += kWave) {
+        const VerifyPart p = pi[(size_t)r * chunks + c];
         if (p.max > m || (p.max == m && p.best < b)) {
           m = p.max;
           b = p.best;
         }
       }
+      // Chunks are in order, so the lowest lane of the maximum has the lowest index (of 64 chunks).
       const float top = verify_max(m);
       b = m == top ? b : 0x7fffffff;
-      for (int off = kWave / 2; off > 0; off >>= 1) b = min(b, __shfl_xor(b, off));
-      if (lane == 0) best[i] = l0 != l0 || b == 0x7fffffff ? 0 : b;  // a NaN at index 0 is never beaten
-    }
-  } else {
-    constexpr int N = 4;
-    for (int i = wave * N; i < a.nodes; i += W * N) {
-      float m[N];
-      double z[N];
-      verify_row<N>(part + (size_t)i * chunks, a.nodes - i, chunks, k2, m, z);
-      if (lane == 0) {
-#pragma unroll
-        for (int r = 0; r < N; r++)
-          if (i + r < a.nodes) {
-            row_max[i + r] = m[r];
-            row_sum[i + r] = z[r];
-          }
+      if (chunks <= kWave) {
+        const uint64_t some = __ballot(b != 0x7fffffff);
+        b = some ? __builtin_amdgcn_readlane(b, __builtin_ctzll(some)) : b;
+      } else {
+        for (int off = kWave / 2; off > 0; off >>= 1) b = min(b, __shfl_xor(b, off));
       }
+      // a NaN at index 0 is never beaten
+      if (lane == 0 && i + r < a.nodes) best[i + r] = l0[r] != l0[r] || b == 0x7fffffff ? 0 : b;
     }
   }
   __syncthreads();
-  if (!greedy && up >= 0) weight[tid] = own.logit == own.logit ? token_weight(own.logit, row_max[up], k2) : 0.0;
-  // Tests that need no more than the row's sums are made for all nodes at once.
-  bool ok = false;
-  if (greedy && up >= 0) ok = token[tid] == best[up];
-  if (point && !greedy) {
-    __syncthreads();
-    bool again = false;  // an earlier sibling has the token: it weighs nothing, as it was rejected there
-    if (up >= 0)
-      for (int j = up + 1; j < tid; j++) again |= parent[j] == up && token[j] == token[tid];
-    __syncthreads();
-    if (again) weight[tid] = 0.0;
-    __syncthreads();
-    if (up >= 0) {
-      double rest = 0.0;  // what is left: the other tokens and the children from here on
-      for (int j = a.nodes - 1; j >= tid; j--) rest += parent[j] == up ? weight[j] : 0.0;
-      ok = uniform[tid] * (row_sum[up] + rest) < weight[tid];
-    }
-  }
-  if (tid < kMaxVerifyNodes) accept[tid] = ok;
-  __syncthreads();
-
-  // The walk, the same in every thread.
   int at = 0, count = 1;
-  bool kids = false;
-  double inv_z = 0.0;
-  VerifyTest t = {0.0, 1.0};
-  int tested = 0;
-  // The sum of max(p - a q, 0) over the row of `at`, by the whole block.
-  auto residual = [&](double ra) {
-    double s = 0.0;
-    const float* row = a.logits + (size_t)at * a.vocab;
-    const float* draft = a.draft + (size_t)at * a.vocab;
-    const bool al = verify_aligned(row), dl = verify_aligned(draft);
-    for (int c = 0; c < chunks; c++) {
-      v4f x[G], q[G];
-      verify_load<kWalkThreads>(row, c * kChunkV, a.vocab, al, NAN, x);
-      verify_load<kWalkThreads>(draft, c * kChunkV, a.vocab, dl, 0.f, q);
-#pragma unroll
-      for (int k = 0; k < 4; k++) s += residual_weight(token_weight(x[0][k], row_max[at], k2), inv_z, ra, q[0][k]);
-    }
-    s = team_sum<64>(s);
-    __syncthreads();
-    if (lane == 0) red[wave] = s;
-    __syncthreads();
-    s = 0.0;
-    for (int w = 0; w < W; w++) s += red[w];
-    return s;
-  };
-  if (!greedy && !point) inv_z = 1.0 / row_sum[0];
   if (tid == 0) a.path[0] = 0;
   for (int i0 = 1; i0 < a.nodes; i0 += kWave) {
-    // The children of `at` among these 64 nodes; a step down goes on with the new node's.
-    const bool here = i0 + lane < a.nodes;
-    const int over = here ? parent[i0 + lane] : -1;
-    uint64_t some = __ballot(over == at);
-    if (greedy || point) {
-      const uint64_t good = __ballot(here && accept[i0 + lane]);
-      kids |= some != 0;
-      while (some & good) {
-        const int i = __builtin_ctzll(some & good);
-        at = i0 + i;
-        if (tid == 0) a.path[count] = at;
-        count++;
-        some = __ballot(over == at);  // all behind i
-        kids = some != 0;
-      }
-      continue;
+    const int i = i0 + lane, over = i < a.nodes ? parent[i] : -1;
+    uint64_t good = __ballot(over == at && token[i] == best[at]);
+    while (good) {
+      at = i0 + __builtin_ctzll(good);
+      if (tid == 0) a.path[count] = at;
+      count++;
+      good = __ballot(over == at && token[i] == best[at]);  // all behind the step
     }
-    while (some) {
-      const int i = i0 + __builtin_ctzll(some);
-      some &= some - 1;
-      if (verify_accept(t, weight[i], inv_z, prob[i], uniform[i])) {
-        at = i;
-        if (tid == 0) a.path[count] = at;
-        count++;
-        tested = 0;
-        t = {0.0, 1.0};
-        inv_z = 1.0 / row_sum[at];
-        some = __ballot(over == at);
-      } else {
-        t.a += t.f;
-        verify_reject(t, tested < rounds ? verify_residual_sum(res + ((size_t)tested * a.nodes + at) * chunks, chunks)
-                                         : residual(t.a));
-        tested++;
-      }
-    }
-  }
-
-  int next = greedy ? best[at] : 0;
-  if (!greedy) {
-    // The chunks' weights: e without the children's tokens (no draft probabilities; all of them if
-    // nothing is left), e (no rejection), or the last residual's.
-    const VerifyPart* pa = part + (size_t)at * chunks;
-    const float m = row_max[at];
-    bool without = point && kids;
-    const bool plain = point || t.a == 0.0;
-    if (without && row_sum[at] == 0.0) without = false;
-    const bool again = point && kids && !without;  // the children's tokens are in no sum: all of the row, once more
-    const double* last = !plain && tested <= rounds ? res + ((size_t)(tested - 1) * a.nodes + at) * chunks : nullptr;
-    const float* row = a.logits + (size_t)at * a.vocab;
-    const float* draft = plain ? nullptr : a.draft + (size_t)at * a.vocab;
-    const bool al = verify_aligned(row), dl = verify_aligned(draft);
-
-    // A chunk's four weights of a thread.
-    auto weigh = [&](int c, double (&w)[4]) {
-      v4f x[G], q[G];
-      verify_load<kWalkThreads>(row, c * kChunkV, a.vocab, al, NAN, x);
-      if (!plain) verify_load<kWalkThreads>(draft, c * kChunkV, a.vocab, dl, 0.f, q);
-      const uint32_t hide = without ? verify_hide<kWalkThreads>(a, at, c * kChunkV, nullptr) : 0u;
-#pragma unroll
-      for (int k = 0; k < 4; k++) {
-        w[k] = token_weight(x[0][k], m, k2);
-        if (!plain) w[k] = residual_weight(w[k], inv_z, t.a, q[0][k]);
-        if (hide >> k & 1) w[k] = 0.0;
-      }
-    };
-    if (again || (!plain && !last)) {  // sums that no launch left
-      for (int c = 0; c < chunks; c++) {
-        double w[4];
-        weigh(c, w);
-        double s = team_sum<64>(w[0] + w[1] + w[2] + w[3]);
-        __syncthreads();
-        if (lane == 0) red[wave] = s;
-        __syncthreads();
-        s = 0.0;
-        for (int k = 0; k < W; k++) s += red[k];
-        if (tid == 0) sums[c] = s;
-      }
-    } else {
-      for (int c = tid; c < chunks; c += kWalkThreads)
-        sums[c] = plain ? pa[c].sum * token_weight(pa[c].max, m, k2) : last[c];
-    }
-    __syncthreads();
-    // The first chunk whose running sum passes the target (every wave for itself, 64 chunks at a time);
-    // where the rounding of the total leaves none, the last one with a weight.
-    double u = uniform[0];
-    u = u > 0.0 ? u : 0.0;
-    if (u >= 1.0) u = 1.0 - 0x1p-53;
-    double total = 0.0;
-    for (int c0 = 0; c0 < chunks; c0 += kWave) total += team_sum<64>(c0 + lane < chunks ? sums[c0 + lane] : 0.0);
-    const double target = u * total;
-    double before = 0.0, run = 0.0;
-    int c = 0;
-    for (int c0 = 0; c0 < chunks; c0 += kWave) {
-      const double own = c0 + lane < chunks ? sums[c0 + lane] : 0.0;
-      const double s = wave_scan(own) + run;
-      const double up = __shfl_up(s, 1), less = lane ? up : run;
-      const uint64_t full = __ballot(own > 0.0), hit = __ballot(own > 0.0 && s > target);
-      const int pick = hit ? __builtin_ctzll(hit) : full ? 63 - __builtin_clzll(full) : -1;
-      if (pick >= 0) {
-        c = c0 + pick;
-        before = __shfl(less, pick);
-      }
-      if (hit) break;
-      run = __shfl(s, kWave - 1);
-    }
-    double w[4];
-    weigh(c, w);
-    const double v = w[0] + w[1] + w[2] + w[3];
-    const double s = wave_scan(v);
-    if (lane == kWave - 1) tail[wave] = s;
-    __syncthreads();
-    double sum = before;
-    for (int k = 0; k < wave; k++) sum += tail[k];
-    sum += s - v;
-    int pick = 0x7fffffff, some = -1;
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-      sum += w[k];
-      if (w[k] > 0.0) {
-        some = c * kChunkV + 4 * tid + k;
-        if (sum > target && pick == 0x7fffffff) pick = some;
-      }
-    }
-    for (int off = kWave / 2; off > 0; off >>= 1) {
-      pick = min(pick, __shfl_xor(pick, off));
-      some = max(some, __shfl_xor(some, off));
-    }
-    if (lane == 0) {
-      wpick[wave] = pick;
-      wsome[wave] = some;
-    }
-    __syncthreads();
-    for (int k = 0; k < W; k++) {
-      pick = min(pick, wpick[k]);
-      some = max(some, wsome[k]);
-    }
-    // Behind the chunk's own rounding: its last token with a weight; 0 where no token has one.
-    next = pick != 0x7fffffff ? pick : some >= 0 ? some : 0;
   }
   if (tid == 0) {
     *a.count = count;
-    *a.next = next;
+    *a.next = best[at];
   }
   if (tid >= count && tid < a.nodes) a.path[tid] = -1;
 }
@@ -630,9 +704,14 @@ hipError_t launch_verify_tree(hipStream_t s, const VerifyArgs& a, void* scratch)
   double* res = reinterpret_cast<double*>(part + (size_t)a.nodes * chunks);
   VerifyKid* kid = reinterpret_cast<VerifyKid*>(res + (size_t)rounds * a.nodes * chunks);
   const dim3 grid(chunks, a.nodes), block(kRowsThreads);
-  if (a.temperature == 0.0) hipLaunchKernelGGL(k_verify_rows<true>, grid, block, 0, s, a, part, kid);
-  else hipLaunchKernelGGL(k_verify_rows<false>, grid, block, 0, s, a, part, kid);
-  for (int r = 0; r < rounds; r++) hipLaunchKernelGGL(k_verify_residual, grid, block, 0, s, a, part, res, r);
+  if (a.temperature == 0.0) {
+    hipLaunchKernelGGL(k_verify_rows<true>, grid, block, 0, s, a, part, kid);
+    hipLaunchKernelGGL(k_verify_walk_greedy, dim3(1), dim3(std::min(kWalkThreads, (a.nodes + 3) / 4 * kWave)), 0, s, a,
+                       part, chunks);
+    return hipGetLastError();
+  }
+  hipLaunchKernelGGL(k_verify_rows<false>, grid, block, 0, s, a, part, kid);
+  for (int r = 0; r < rounds; r++) hipLaunchKernelGGL(k_verify_residual, grid, block, 0, s, a, part, kid, res, r);
   hipLaunchKernelGGL(k_verify_walk, dim3(1), dim3(kWalkThreads), 0, s, a, part, kid, res, rounds, chunks);
   return hipGetLastError();
 }
