@@ -18,6 +18,7 @@
 // through LDS in order. Ranges of a long context go to blocks of their own (grid x), whose states a
 // second launch merges in order.
 #include <algorithm>
+#include <cmath>
 
 #include "attention.h"
 
@@ -26,7 +27,6 @@ namespace qh {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int kTreeCols = 32;    // rows of a wave's tile
 constexpr int kTreeKeys = 32;    // keys of a step
-constexpr int kTreePart = 68;    // floats of a row's partial: m, l, 2 pad, o[64]
 constexpr int kMaxTreeSplits = 128;
 constexpr float kWeightLog2 = 15.f;  // p is held as 2^15 p
 
@@ -49,13 +49,6 @@ __device__ __forceinline__ uint32_t tree_window(const uint64_t* mask, int words,
   }
   const int n = nodes - j0;  // > 0: the step starts before the last node
   return n < 32 ? win & ((1u << n) - 1u) : win;
-}
-
-__device__ __forceinline__ bool f16_pair_odd(uint32_t u) {  // either half infinite or NaN
-  return (u & 0x7c00u) == 0x7c00u || (u & 0x7c000000u) == 0x7c000000u;
-}
-__device__ __forceinline__ uint32_t f16_pair_finite(uint32_t u) {  // such halves as zero
-  return ((u & 0x7c00u) == 0x7c00u ? 0u : u & 0xffffu) | ((u & 0x7c000000u) == 0x7c000000u ? 0u : u & 0xffff0000u);
 }
 
 __device__ __forceinline__ void tree_load_k(const uint16_t* kb, int p0, int capacity, int col, int hb, f16x8 (&k)[4]) {
@@ -166,204 +159,281 @@ __device__ __forceinline__ void tree_hide(f32x16& s, uint32_t win, int hb) {
   for (int i = 0; i < 16; i++) s[i] = mine >> (16 * (i / 8) + i % 8) & 1 ? s[i] : -INFINITY;
 }
 
-// A value operand of keys k0 .. k0+7 without what must not reach a product: positions from `total` on,
-// which hold whatever the cache holds. True: some value left is infinite or NaN.
-__device__ __forceinline__ bool tree_clip(v4u& v, int k0, int total) {
-  bool odd = false;
+// A value operand of keys k0 .. k0+7 with positions from `total` on, which hold whatever the cache holds, as zeros.
+__device__ __forceinline__ void tree_clip(v4u& v, int k0, int total) {
 #pragma unroll
-  for (int w = 0; w < 4; w++) {
+  for (int w = 0; w < 4; w++)
     v[w] &= (k0 + 2 * w < total ? 0x0000ffffu : 0u) | (k0 + 2 * w + 1 < total ? 0xffff0000u : 0u);
-    odd |= f16_pair_odd(v[w]);
-  }
-  return odd;
 }
 
-// What infinite and NaN values at p0 .. p0+31 add to the rows that see them. In the products they
-// are zeros: there they would reach every row, as 0 * inf.
-__device__ __forceinline__ void tree_add_odd(const uint16_t* vb, int vstride, int p0, int total, uint32_t win, int hb,
-                                          f32x16 (&o)[2]) {
-#pragma unroll 1
-  for (int k = 0; k < kTreeKeys && p0 + k < total; k++) {
-    const bool sees = win >> k & 1;
-#pragma unroll
-    for (int dt = 0; dt < 2; dt++)
-#pragma unroll
-      for (int i = 0; i < 16; i++) {
-        const uint16_t v = vb[(size_t)(32 * dt + 8 * (i / 4) + 4 * hb + i % 4) * vstride + p0 + k];
-        if (sees && (v & 0x7c00u) == 0x7c00u) o[dt][i] += (float)__builtin_bit_cast(_Float16, v);
-      }
-  }
-}
-
-// A row's state to its output (one split) or its partial.
-__device__ __forceinline__ void tree_store(const TreeAttnArgs& a, float* part, size_t at, int split, int splits, int hb, float m,
-                                           float l, f32x16 (&o)[2]) {
-  float* dst;
-  if (splits == 1) {
-    dst = a.out + at * kHeadDim;
-    const float inv = 1.f / l;
-#pragma unroll
-    for (int dt = 0; dt < 2; dt++)
-#pragma unroll
-      for (int i = 0; i < 16; i++) o[dt][i] = l == 0.f ? 0.f : o[dt][i] * inv;
-  } else {
-    float* p = part + (at * splits + split) * kTreePart;
-    if (hb == 0) {
-      p[0] = m;
-      p[1] = l;
-    }
-    dst = p + 4;
-  }
+__device__ __forceinline__ bool tree_odd(const f32x16 (&o)[2]) {
+  float z = 0.f;
 #pragma unroll
   for (int dt = 0; dt < 2; dt++)
 #pragma unroll
-    for (int i = 0; i < 16; i += 4)
-      *reinterpret_cast<v4f*>(dst + 32 * dt + 2 * i + 4 * hb) = v4f{o[dt][i], o[dt][i + 1], o[dt][i + 2], o[dt][i + 3]};
+    for (int i = 0; i < 16; i++) z = fmaf(o[dt][i], 0.f, z);
+  return __any(z != 0.f);
 }
 
-// Few rows: each wave takes its keys straight from the cache. Block of WQ x WK waves, WQ column tiles
-// by WK runs of keys: wave (t, k) takes the 32-key steps k, k + WK, ... of the block's range for tile t,
-// the next step's loads in flight, and the WK states of a tile merge through LDS in order.
-template <int WQ, int WK>
-__global__ __launch_bounds__(kWave * WQ * WK, 2) void k_attn_tree_few(TreeAttnArgs a, float* __restrict__ part) {
-  constexpr int kMerge = WK > 1 ? WK - 1 : 1;
-  __shared__ float sh_o[kMerge][WQ][32][kWave];
-  __shared__ float sh_m[kMerge][WQ][kTreeCols], sh_l[kMerge][WQ][kTreeCols];
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, wq = wave % WQ, wk = wave / WQ;
+// Where a row's partial lies: rows in the order of the tiles, kv head by kv head.
+__device__ __forceinline__ size_t tree_slot(int kvh, int rows, int row, int kv_heads, int split) {
+  return ((size_t)split * kv_heads + kvh) * rows + row;
+}
+
+// Infinite and NaN values reach every row of a product, as 0 * inf, seen or not. So a block whose output is not
+// finite does its keys once more with care: such values of the nodes are zeros in the products (which
+// changes no bit of the rows that do not see them), and afterwards the rows that do get them here:
+// rows row0 + first, + step, ... of a tile, lane d dimension d, keys k0 .. k1-1.
+__device__ __forceinline__ uint32_t f16_pair_finite(uint32_t u) {
+  return ((u & 0x7c00u) == 0x7c00u ? 0u : u & 0xffffu) | ((u & 0x7c000000u) == 0x7c000000u ? 0u : u & 0xffff0000u);
+}
+// tree_clip, with infinite and NaN values from position `from` on as zeros too.
+__device__ __forceinline__ void tree_clip(v4u& v, int k0, int total, int from) {
+  tree_clip(v, k0, total);
+#pragma unroll
+  for (int w = 0; w < 4; w++) {
+    const uint32_t f = f16_pair_finite(v[w]);
+    v[w] = (k0 + 2 * w < from ? v[w] & 0xffffu : f & 0xffffu) | (k0 + 2 * w + 1 < from ? v[w] & 0xffff0000u : f & 0xffff0000u);
+  }
+}
+__device__ __noinline__ void tree_add_odd(TreeAttnArgs a, float* part, int kvh, int row0, int first, int step, int k0, int k1,
+                                          int split, int splits) {
+  const int lane = threadIdx.x & (kWave - 1), group = a.heads / a.kv_heads, rows = a.nodes * group;
+  const uint16_t* vb = a.vt + ((size_t)kvh * kHeadDim + lane) * a.vstride;
+  for (int row = row0 + first; row < min(row0 + kTreeCols, rows); row += step) {
+    const int node = row / group;
+    const uint64_t* mask = a.mask + (size_t)node * ((a.nodes + 63) / 64);
+    float acc = 0.f;
+    bool any = false;
+#pragma unroll 1
+    for (int k = max(k0, a.past); k < k1; k++) {
+      const int j = k - a.past;
+      if (!(mask[j >> 6] >> (j & 63) & 1)) continue;
+      const uint16_t v = vb[k];
+      if ((v & 0x7c00u) != 0x7c00u) continue;
+      acc += (float)__builtin_bit_cast(_Float16, v);
+      any = true;
+    }
+    if (!any) continue;
+    float* dst = splits > 1 ? part + tree_slot(kvh, rows, row, a.kv_heads, split) * kHeadDim
+                            : a.out + ((size_t)node * a.heads + kvh * group + row % group) * kHeadDim;
+    dst[lane] = acc;
+  }
+}
+
+// A tile's states to their outputs (one split) or partials, through `buf` (LDS of the wave's own), so that a store
+// is whole rows: 8 x 1 KB (in 32-byte pieces the partials of 64 ranges of 896 rows took 7 us more).
+constexpr int kStoreRow = kHeadDim + 4;  // floats
+__device__ __forceinline__ void tree_store(const TreeAttnArgs& a, float* part, float* part_ml, float* buf, int kvh, int row0,
+                                           int split, int splits, int lane, float m, float l, f32x16 (&o)[2]) {
+  const int col = lane & 31, hb = lane >> 5, group = a.heads / a.kv_heads, rows = a.nodes * group;
+  const float scale = splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int g = 0; g < 8; g++) {
+    const int dt = g / 4, i = 4 * (g % 4);
+    v4f x = {o[dt][i], o[dt][i + 1], o[dt][i + 2], o[dt][i + 3]};
+#pragma unroll
+    for (int r = 0; r < 4; r++) x[r] *= scale;
+    *reinterpret_cast<v4f*>(buf + col * kStoreRow + 32 * dt + 8 * (g % 4) + 4 * hb) = x;
+  }
+  const size_t slot = tree_slot(kvh, rows, row0, a.kv_heads, split);
+  if (splits > 1 && hb == 0 && row0 + col < rows) *reinterpret_cast<f32x2*>(part_ml + 2 * (slot + col)) = f32x2{m, l};
+  wave_lds_handoff();
+#pragma unroll 2
+  for (int k = 0; k < 8; k++) {
+    const int r = 4 * k + (lane >> 4), row = row0 + r;
+    const v4f x = *reinterpret_cast<const v4f*>(buf + r * kStoreRow + 4 * (lane & 15));
+    if (row >= rows) continue;
+    float* dst = splits > 1 ? part + (slot + r) * kHeadDim
+                            : a.out + ((size_t)(row / group) * a.heads + kvh * group + row % group) * kHeadDim;
+    *reinterpret_cast<v4f*>(dst + 4 * (lane & 15)) = x;
+  }
+}
+
+// Short contexts and few rows: each wave takes its keys straight from the cache. A block of WK waves has a
+// tile of rows and a range of keys; wave w takes the 32-key steps w, w + WK, ... of it, the next step's
+// loads in flight, and the waves' states merge through LDS, each wave merging its share of the dimensions
+// over all of them in order.
+template <int WK>
+__global__ __launch_bounds__(kWave * WK, 2) void k_attn_tree_direct(TreeAttnArgs a, float* __restrict__ part, float* __restrict__ part_ml) {
+  constexpr int kGroups = 8;  // of four dimensions: 32 (g / 4) + 8 (g % 4) + 4 hb .. +3
+  __shared__ v4f sh_o[WK][kGroups][kWave];
+  __shared__ float sh_m[WK][kTreeCols], sh_l[WK][kTreeCols];
+  const int lane = threadIdx.x & (kWave - 1), wk = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int col = lane & 31, hb = lane >> 5;
   const int group = a.heads / a.kv_heads, rows = a.nodes * group;
   const int kvh = blockIdx.z, total = a.past + a.nodes, words = (a.nodes + 63) / 64;
-  const int tile = blockIdx.y * WQ + wq;
-  const int row = min(tile * kTreeCols + col, rows - 1);  // past the end, a copy of the last
+  const int row = min((int)blockIdx.y * kTreeCols + col, rows - 1);  // past the end, a copy of the last
   const int node = row / group, head = kvh * group + row % group;
   const uint16_t* kb = a.kc + (size_t)kvh * a.capacity * kHeadDim;
   const uint16_t* vb = a.vt + (size_t)kvh * kHeadDim * a.vstride;
   const uint64_t* mask = a.mask + (size_t)node * words;
   const int steps = (total + kTreeKeys - 1) / kTreeKeys;
-  // a tile past the last row has nothing to do but meet the barrier
-  const int end = tile * kTreeCols < rows ? tree_part(steps, blockIdx.x + 1, gridDim.x) : 0;
-  int step = tree_part(steps, blockIdx.x, gridDim.x) + wk;
+  const int first = tree_part(steps, blockIdx.x, gridDim.x) + wk, end = tree_part(steps, blockIdx.x + 1, gridDim.x);
 
   f16x8 kf[4];
   v4u vf[2][2];
-  if (step < end) {
-    tree_load_k(kb, step * kTreeKeys, a.capacity, col, hb, kf);
-    tree_load_v(vb, step * kTreeKeys, a.vstride, col, hb, vf);
+  uint32_t win, next_win = 0xffffffffu;
+  auto look = [&](int step) {
+    const int p0 = step * kTreeKeys;
+    next_win = p0 + kTreeKeys > a.past ? tree_window(mask, words, a.nodes, a.past, p0) : 0xffffffffu;
+  };
+  if (first < end) {
+    tree_load_k(kb, first * kTreeKeys, a.capacity, col, hb, kf);
+    tree_load_v(vb, first * kTreeKeys, a.vstride, col, hb, vf);
+    look(first);
   }
   f16x8 qh[4], ql[4];
   const size_t at = (size_t)node * a.heads + head;
   const float c = tree_query(a.q + at * kHeadDim + 8 * hb, qh, ql);
-  float m = -INFINITY, l = 0.f;
-  f32x16 o[2];
-#pragma unroll
-  for (int dt = 0; dt < 2; dt++)
-#pragma unroll
-    for (int i = 0; i < 16; i++) o[dt][i] = 0.f;
-
-  for (; step < end; step += WK) {
-    const int p0 = step * kTreeKeys, next = min(step + WK, steps - 1) * kTreeKeys;
-    f32x16 s[1];
-#pragma unroll
-    for (int i = 0; i < 16; i++) s[0][i] = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < 4; ks++) s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[ks], qh[ks], s[0], 0, 0, 0);
-#pragma unroll
-    for (int ks = 0; ks < 4; ks++) s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[ks], ql[ks], s[0], 0, 0, 0);
-    tree_load_k(kb, next, a.capacity, col, hb, kf);
-    const bool masked = p0 + kTreeKeys > a.past;  // uniform
-    uint32_t win = 0xffffffffu;
-    if (masked) {
-      win = tree_window(mask, words, a.nodes, a.past, p0);
-      tree_hide(s[0], win, hb);
-    }
-    tree_max(s, c, m, l, o);
-    f16x8 ph[2], pl[2];
-    tree_weights(s[0], c, m, l, ph, pl);
-    bool odd = false;
-    if (masked) {
-#pragma unroll
-      for (int dt = 0; dt < 2; dt++)
-#pragma unroll
-        for (int ks = 0; ks < 2; ks++) odd |= tree_clip(vf[dt][ks], p0 + 16 * ks + 8 * hb, total);
-      odd = __any(odd);
-      if (odd) {
-#pragma unroll
-        for (int dt = 0; dt < 2; dt++)
-#pragma unroll
-          for (int ks = 0; ks < 2; ks++)
-#pragma unroll
-            for (int w = 0; w < 4; w++) vf[dt][ks][w] = f16_pair_finite(vf[dt][ks][w]);
-      }
-    }
-#pragma unroll
-    for (int ks = 0; ks < 2; ks++)
-#pragma unroll
-      for (int dt = 0; dt < 2; dt++) {
-        const f16x8 va = __builtin_bit_cast(f16x8, vf[dt][ks]);
-        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph[ks], o[dt], 0, 0, 0);
-        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl[ks], o[dt], 0, 0, 0);
-      }
-    tree_load_v(vb, next, a.vstride, col, hb, vf);
-    if (odd) tree_add_odd(vb, a.vstride, p0, total, win, hb, o);
-  }
-  l = pair_sum(l);
-
-  if constexpr (WK > 1) {
-    if (wk > 0) {
-#pragma unroll
-      for (int dt = 0; dt < 2; dt++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) sh_o[wk - 1][wq][16 * dt + i][lane] = o[dt][i];
-      if (hb == 0) {
-        sh_m[wk - 1][wq][col] = m;
-        sh_l[wk - 1][wq][col] = l;
-      }
-    }
-    __syncthreads();
-    if (wk > 0) return;
-    float mx = m;
-#pragma unroll
-    for (int w = 0; w < WK - 1; w++) mx = fmaxf(mx, sh_m[w][wq][col]);
-    const float own = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mx);
-    l *= own;
+  __shared__ float sh_out[kTreeCols][kStoreRow];
+  float m, l, mx;
+  bool care = false;
+  for (;; care = true) {
+    m = -INFINITY;
+    l = 0.f;
+    f32x16 o[2];
 #pragma unroll
     for (int dt = 0; dt < 2; dt++)
 #pragma unroll
-      for (int i = 0; i < 16; i++) o[dt][i] *= own;
+      for (int i = 0; i < 16; i++) o[dt][i] = 0.f;
+    for (int step = first; step < end; step += WK) {
+      const int p0 = step * kTreeKeys;
+      const bool more = step + WK < end;
+      f32x16 s[1];
 #pragma unroll
-    for (int w = 0; w < WK - 1; w++) {
-      const float mw = sh_m[w][wq][col];
-      const float wt = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - mx);
-      l = fmaf(sh_l[w][wq][col], wt, l);
+      for (int i = 0; i < 16; i++) s[0][i] = 0.f;
 #pragma unroll
-      for (int dt = 0; dt < 2; dt++)
+      for (int ks = 0; ks < 4; ks++) s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[ks], qh[ks], s[0], 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < 16; i++) o[dt][i] = fmaf(sh_o[w][wq][16 * dt + i][lane], wt, o[dt][i]);
+      for (int ks = 0; ks < 4; ks++) s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[ks], ql[ks], s[0], 0, 0, 0);
+      win = next_win;
+      if (more) {
+        tree_load_k(kb, p0 + WK * kTreeKeys, a.capacity, col, hb, kf);
+        look(step + WK);
+      }
+      if (p0 + kTreeKeys > a.past) tree_hide(s[0], win, hb);  // uniform
+      tree_max(s, c, m, l, o);
+      f16x8 ph[2], pl[2];
+      tree_weights(s[0], c, m, l, ph, pl);
+      if (p0 + kTreeKeys > total) {
+#pragma unroll
+        for (int dt = 0; dt < 2; dt++)
+#pragma unroll
+          for (int ks = 0; ks < 2; ks++) tree_clip(vf[dt][ks], p0 + 16 * ks + 8 * hb, total);
+      }
+      if (care) {
+#pragma unroll
+        for (int dt = 0; dt < 2; dt++)
+#pragma unroll
+          for (int ks = 0; ks < 2; ks++) tree_clip(vf[dt][ks], p0 + 16 * ks + 8 * hb, total, a.past);
+      }
+#pragma unroll
+      for (int ks = 0; ks < 2; ks++) {
+#pragma unroll
+        for (int dt = 0; dt < 2; dt++)
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, vf[dt][ks]), ph[ks], o[dt], 0, 0, 0);
+#pragma unroll
+        for (int dt = 0; dt < 2; dt++)
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, vf[dt][ks]), pl[ks], o[dt], 0, 0, 0);
+      }
+      if (more) tree_load_v(vb, p0 + WK * kTreeKeys, a.vstride, col, hb, vf);
     }
-    m = mx;
+    l = pair_sum(l);
+
+#pragma unroll
+    for (int g = 0; g < kGroups; g++) {
+      const int dt = g / 4, i = 4 * (g % 4);
+      sh_o[wk][g][lane] = v4f{o[dt][i], o[dt][i + 1], o[dt][i + 2], o[dt][i + 3]};
+    }
+    if (hb == 0) {
+      sh_m[wk][col] = m;
+      sh_l[wk][col] = l;
+    }
+    __syncthreads();
+    // Each wave merges its share of the dimensions; the tile's rows leave through LDS.
+    float wt[WK];
+    mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WK; w++) {
+      wt[w] = sh_m[w][col];
+      mx = fmaxf(mx, wt[w]);
+    }
+    l = 0.f;
+#pragma unroll
+    for (int w = 0; w < WK; w++) {
+      wt[w] = wt[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(wt[w] - mx);
+      l = fmaf(sh_l[w][col], wt[w], l);
+    }
+    const float scale = gridDim.x > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+    float z = 0.f;
+#pragma unroll
+    for (int k = 0; k < kGroups / WK; k++) {
+      const int g = wk * (kGroups / WK) + k;
+      v4f x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < WK; w++) {
+        const v4f y = sh_o[w][g][lane];
+#pragma unroll
+        for (int r = 0; r < 4; r++) x[r] = fmaf(y[r], wt[w], x[r]);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        z = fmaf(x[r], 0.f, z);
+        x[r] *= scale;
+      }
+      *reinterpret_cast<v4f*>(&sh_out[col][32 * (g / 4) + 8 * (g % 4) + 4 * hb]) = x;
+    }
+    if (!__syncthreads_or(z != 0.f) || care) break;
+    if (first < end) {
+      tree_load_k(kb, first * kTreeKeys, a.capacity, col, hb, kf);
+      tree_load_v(vb, first * kTreeKeys, a.vstride, col, hb, vf);
+      look(first);
+    }
   }
-  if (tile * kTreeCols + col < rows) tree_store(a, part, at, blockIdx.x, gridDim.x, hb, m, l, o);
+  const int row0 = blockIdx.y * kTreeCols;
+  const size_t slot = tree_slot(kvh, rows, row0, a.kv_heads, blockIdx.x);
+  if (gridDim.x > 1 && wk == 0 && hb == 0 && row0 + col < rows) *reinterpret_cast<f32x2*>(part_ml + 2 * (slot + col)) = f32x2{mx, l};
+  for (int i = threadIdx.x; i < kTreeCols * 16; i += kWave * WK) {
+    const int r = i >> 4;
+    if (row0 + r >= rows) break;
+    float* dst = gridDim.x > 1 ? part + (slot + r) * kHeadDim
+                               : a.out + ((size_t)((row0 + r) / group) * a.heads + kvh * group + (row0 + r) % group) * kHeadDim;
+    *reinterpret_cast<v4f*>(dst + 4 * (i & 15)) = *reinterpret_cast<const v4f*>(&sh_out[r][4 * (i & 15)]);
+  }
+  if (care) {
+    __syncthreads();
+    tree_add_odd(a, part, kvh, row0, wk, WK, kTreeKeys * tree_part(steps, blockIdx.x, gridDim.x), min(kTreeKeys * end, total), blockIdx.x,
+                 gridDim.x);
+  }
 }
 
-// Many rows: a block's W waves, a column tile each, share tiles of 64 keys (whole 128-byte lines of both
-// caches) staged in LDS, the next one in flight while the current one is used. LDS rows are 128 bytes,
-// K's in tree_key's order; their 16-byte pieces are stored at piece ^ (row % 8), so that the 8 lanes
-// of a read phase, which want the same piece of 8 rows, find it in different banks.
+// Long contexts and many rows: a block's waves, a column tile each, share stages of 64 keys (whole 128-byte
+// lines of both caches) in LDS. LDS rows are 128 bytes, K's in tree_key's order; their 16-byte pieces are stored
+// at piece ^ (row / 2 % 8), so that the 16 lanes of a read's cycle, which want one piece of 16 rows, find it in
+// different banks. A stage's scores are made while the weights of the one before it are: its K is
+// staged one turn ahead of its V, and the products' matrix instructions have the exponentials to run under.
 constexpr int kTreeStage = 64;
-constexpr int kTreeWaves = 4;
+constexpr int kTreeWaves = 8;
 
-// The copies of one stage, 16 of 1 KB (8 rows of K or of V each, 16 bytes a lane), dealt to the waves. They
-// land on their own (vmcnt), so whoever reads them waits with tree_landed and meets the other waves.
-__device__ __forceinline__ void tree_stage(const uint16_t* kb, const uint16_t* vb, int p0, int capacity, int vstride, int wave,
-                                           int waves, int lane, uint16_t (&buf)[2][kTreeStage * kHeadDim]) {
-  const int sub = lane >> 3;
+// The copies of one stage of K or V, 8 of 1 KB (8 rows each, 16 bytes a lane), dealt to the waves. They land on
+// their own (vmcnt), so whoever reads them waits with tree_landed and meets the other waves. In asm, as the
+// compiler would have every later read of LDS wait for them, also one of another stage. `to` is
+// uniform; lane l's 16 bytes land at to + 16 l.
+__device__ __forceinline__ void copy_to_lds(const uint16_t* from, uint16_t* to) {
+  const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)to);
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory", "m0");
+}
+__device__ __forceinline__ void tree_stage_k(const uint16_t* kb, int p0, int capacity, int wave, int waves, int lane, uint16_t* buf) {
   for (int j = wave; j < 8; j += waves) {
-    const int r = 8 * j + sub, piece = (lane & 7) ^ (sub & 7);
-    __builtin_amdgcn_global_load_lds(
-        (const __attribute__((address_space(1))) void*)(kb + (size_t)min(p0 + (r & 32) + tree_key(r & 31), capacity - 1) * kHeadDim + 8 * piece),
-        (__attribute__((address_space(3))) void*)&buf[0][j * 512], 16, 0, 0);
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(vb + (size_t)r * vstride + p0 + 8 * piece),
-                                     (__attribute__((address_space(3))) void*)&buf[1][j * 512], 16, 0, 0);
+    const int r = 8 * j + (lane >> 3), piece = (lane & 7) ^ (r >> 1 & 7);
+    copy_to_lds(kb + (size_t)min(p0 + (r & 32) + tree_key(r & 31), capacity - 1) * kHeadDim + 8 * piece, buf + j * 512);
+  }
+}
+__device__ __forceinline__ void tree_stage_v(const uint16_t* vb, int p0, int vstride, int wave, int waves, int lane, uint16_t* buf) {
+  for (int j = wave; j < 8; j += waves) {
+    const int r = 8 * j + (lane >> 3), piece = (lane & 7) ^ (r >> 1 & 7);
+    copy_to_lds(vb + (size_t)r * vstride + p0 + 8 * piece, buf + j * 512);
   }
 }
 __device__ __forceinline__ void tree_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
@@ -375,11 +445,12 @@ struct TreeTile {
   f32x16 o[2];
 };
 
-// One stage of 64 keys for a wave's tile. MASKED: some of its keys are nodes or lie behind the last one.
-template <bool MASKED>
-__device__ __forceinline__ void tree_use(const uint16_t (&cur)[2][kTreeStage * kHeadDim], TreeTile& t, int col, int hb, int p0,
-                                         const TreeAttnArgs& a, const uint64_t* mask, const uint16_t* vb) {
-  f32x16 s[2];
+// The operand of 16-byte piece `piece` of LDS row 32 half + col.
+__device__ __forceinline__ v4u tree_piece(const uint16_t* buf, int half, int col, int piece) {
+  return *reinterpret_cast<const v4u*>(buf + (32 * half + col) * kTreeStage + 8 * (piece ^ (col >> 1 & 7)));
+}
+
+__device__ __forceinline__ void tree_scores(const uint16_t* kbuf, const TreeTile& t, int col, int hb, f32x16 (&s)[2]) {
 #pragma unroll
   for (int j = 0; j < 2; j++)
 #pragma unroll
@@ -388,59 +459,106 @@ __device__ __forceinline__ void tree_use(const uint16_t (&cur)[2][kTreeStage * k
   for (int ks = 0; ks < 4; ks++) {
     f16x8 kf[2];
 #pragma unroll
-    for (int j = 0; j < 2; j++)
-      kf[j] = *reinterpret_cast<const f16x8*>(&cur[0][(32 * j + col) * kHeadDim + 8 * ((2 * ks + hb) ^ (col & 7))]);
+    for (int j = 0; j < 2; j++) kf[j] = __builtin_bit_cast(f16x8, tree_piece(kbuf, j, col, 2 * ks + hb));
 #pragma unroll
     for (int j = 0; j < 2; j++) s[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[j], t.qh[ks], s[j], 0, 0, 0);
 #pragma unroll
     for (int j = 0; j < 2; j++) s[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[j], t.ql[ks], s[j], 0, 0, 0);
   }
+}
+
+// The stage of scores s into the tile's state, where some of its keys may be nodes or lie behind the last one.
+__device__ __forceinline__ void tree_take(const uint16_t* vbuf, TreeTile& t, f32x16 (&s)[2], int col, int hb, int p0,
+                                          const TreeAttnArgs& a, const uint64_t* mask) {
   const int total = a.past + a.nodes;
-  uint32_t win[2];
-  if constexpr (MASKED) {
+  {
 #pragma unroll
     for (int j = 0; j < 2; j++) {
       const int q0 = p0 + 32 * j;
-      win[j] = q0 + 32 <= a.past ? 0xffffffffu : q0 < total ? tree_window(mask, (a.nodes + 63) / 64, a.nodes, a.past, q0) : 0u;
-      tree_hide(s[j], win[j], hb);
+      const uint32_t win = q0 + 32 <= a.past ? 0xffffffffu : q0 < total ? tree_window(mask, (a.nodes + 63) / 64, a.nodes, a.past, q0) : 0u;
+      tree_hide(s[j], win, hb);
     }
   }
   tree_max(s, t.c, t.m, t.l, t.o);
-  bool odd = false;
 #pragma unroll
   for (int j = 0; j < 2; j++) {
     f16x8 ph[2], pl[2];
     tree_weights(s[j], t.c, t.m, t.l, ph, pl);
 #pragma unroll
     for (int ks = 0; ks < 2; ks++) {
-      f16x8 va[2];
+      v4u v[2];
 #pragma unroll
       for (int dt = 0; dt < 2; dt++) {
-        v4u v = *reinterpret_cast<const v4u*>(&cur[1][(32 * dt + col) * kTreeStage + 8 * ((4 * j + 2 * ks + hb) ^ (col & 7))]);
-        if constexpr (MASKED) {
-          odd |= tree_clip(v, p0 + 32 * j + 16 * ks + 8 * hb, total);
-#pragma unroll
-          for (int w = 0; w < 4; w++) v[w] = f16_pair_finite(v[w]);
-        }
-        va[dt] = __builtin_bit_cast(f16x8, v);
+        v[dt] = tree_piece(vbuf, dt, col, 4 * j + 2 * ks + hb);
+        tree_clip(v[dt], p0 + 32 * j + 16 * ks + 8 * hb, total);
       }
 #pragma unroll
-      for (int dt = 0; dt < 2; dt++) t.o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[dt], ph[ks], t.o[dt], 0, 0, 0);
+      for (int dt = 0; dt < 2; dt++)
+        t.o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, v[dt]), ph[ks], t.o[dt], 0, 0, 0);
 #pragma unroll
-      for (int dt = 0; dt < 2; dt++) t.o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[dt], pl[ks], t.o[dt], 0, 0, 0);
-    }
-  }
-  if constexpr (MASKED) {
-    if (__any(odd)) {
-#pragma unroll
-      for (int j = 0; j < 2; j++) tree_add_odd(vb, a.vstride, p0 + 32 * j, total, win[j], hb, t.o);
+      for (int dt = 0; dt < 2; dt++)
+        t.o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, v[dt]), pl[ks], t.o[dt], 0, 0, 0);
     }
   }
 }
 
-__global__ __launch_bounds__(kWave * kTreeWaves, 2) void k_attn_tree_many(TreeAttnArgs a, int splits, int tiles,
-                                                                        float* __restrict__ part) {
-  __shared__ __attribute__((aligned(16))) uint16_t buf[2][2][kTreeStage * kHeadDim];
+// A stage in the past and the scores of the one after it, in one run of code without a branch, so that the
+// matrix instructions of the scores run under the exponentials of the first half and those of the first
+// half's values under the second's.
+__device__ __forceinline__ void tree_step(const uint16_t* kbuf, const uint16_t* vbuf, TreeTile& t, const f32x16 (&s)[2],
+                                          f32x16 (&next)[2], int col, int hb) {
+  f16x8 kf[4][2];
+#pragma unroll
+  for (int ks = 0; ks < 4; ks++)
+#pragma unroll
+    for (int j = 0; j < 2; j++) kf[ks][j] = __builtin_bit_cast(f16x8, tree_piece(kbuf, j, col, 2 * ks + hb));
+  float big = s[0][0];
+#pragma unroll
+  for (int j = 0; j < 2; j++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) big = fmaxf(big, s[j][i]);
+  const float mn = fmaxf(t.m, pair_max(big) * t.c);
+  const float alpha = __builtin_amdgcn_exp2f(t.m - mn);  // 0 from -inf; the scores of the past are finite or NaN
+  t.m = mn;
+  t.l *= alpha;
+#pragma unroll
+  for (int dt = 0; dt < 2; dt++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) t.o[dt][i] *= alpha;
+#pragma unroll
+  for (int j = 0; j < 2; j++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) next[j][i] = 0.f;
+#pragma unroll
+  for (int j = 0; j < 2; j++) {
+#pragma unroll
+    for (int ks = 2 * j; ks < 2 * j + 2; ks++) {
+#pragma unroll
+      for (int e = 0; e < 2; e++) next[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[ks][e], t.qh[ks], next[e], 0, 0, 0);
+#pragma unroll
+      for (int e = 0; e < 2; e++) next[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[ks][e], t.ql[ks], next[e], 0, 0, 0);
+    }
+    f16x8 ph[2], pl[2];
+    tree_weights(s[j], t.c, t.m, t.l, ph, pl);
+#pragma unroll
+    for (int ks = 0; ks < 2; ks++) {
+      v4u v[2];
+#pragma unroll
+      for (int dt = 0; dt < 2; dt++) v[dt] = tree_piece(vbuf, dt, col, 4 * j + 2 * ks + hb);
+#pragma unroll
+      for (int dt = 0; dt < 2; dt++)
+        t.o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, v[dt]), ph[ks], t.o[dt], 0, 0, 0);
+#pragma unroll
+      for (int dt = 0; dt < 2; dt++)
+        t.o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, v[dt]), pl[ks], t.o[dt], 0, 0, 0);
+    }
+  }
+}
+
+__global__ __launch_bounds__(kWave * kTreeWaves, 2) void k_attn_tree_staged(TreeAttnArgs a, int splits, int tiles,
+                                                                          float* __restrict__ part, float* __restrict__ part_ml) {
+  __shared__ __attribute__((aligned(16))) uint16_t kbuf[2][kTreeStage * kHeadDim], vbuf[2][kTreeStage * kHeadDim];
+  __shared__ __attribute__((aligned(16))) float out_buf[kTreeWaves][kTreeCols * kStoreRow];
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int waves = blockDim.x / kWave, col = lane & 31, hb = lane >> 5;
   // Block b runs on XCD b % 8: where the ranges can be dealt to the XCDs evenly, those that share a range
@@ -459,61 +577,86 @@ __global__ __launch_bounds__(kWave * kTreeWaves, 2) void k_attn_tree_many(TreeAt
   const int stages = (total + kTreeStage - 1) / kTreeStage;
   const int first = tree_part(stages, split, splits), end = tree_part(stages, split + 1, splits);
   const int clear = min(end, a.past / kTreeStage);  // the stages before it are all in the past
-  const bool mine = tile * kTreeCols < rows;
 
-  tree_stage(kb, vb, first * kTreeStage, a.capacity, a.vstride, wave, waves, lane, buf[0]);
+  tree_stage_k(kb, first * kTreeStage, a.capacity, wave, waves, lane, kbuf[0]);
   TreeTile t;
-  const size_t at = (size_t)node * a.heads + head;
-  t.c = tree_query(a.q + at * kHeadDim + 8 * hb, t.qh, t.ql);
-  t.m = -INFINITY;
-  t.l = 0.f;
+  t.c = tree_query(a.q + ((size_t)node * a.heads + head) * kHeadDim + 8 * hb, t.qh, t.ql);
+  const bool mine = tile * kTreeCols < rows;
+  bool care = false;
+  for (;; care = true) {
+    t.m = -INFINITY;
+    t.l = 0.f;
 #pragma unroll
-  for (int dt = 0; dt < 2; dt++)
+    for (int dt = 0; dt < 2; dt++)
 #pragma unroll
-    for (int i = 0; i < 16; i++) t.o[dt][i] = 0.f;
-
-  // A stage has landed when every wave has passed the barrier, and every wave is done with the other buffer.
-  auto turn = [&](int st) -> int {
+      for (int i = 0; i < 16; i++) t.o[dt][i] = 0.f;
     tree_landed();
     __syncthreads();
-    const int now = (st - first) & 1;
-    if (st + 1 < end)
-      tree_stage(kb, vb, (st + 1) * kTreeStage, a.capacity, a.vstride, wave, waves, lane, buf[now ^ 1]);
-    return now;
-  };
-  int st = first;
-  for (; st < clear; st++) {
-    const int now = turn(st);
-    if (mine) tree_use<false>(buf[now], t, col, hb, st * kTreeStage, a, mask, vb);
+    if (first + 1 < end) tree_stage_k(kb, (first + 1) * kTreeStage, a.capacity, wave, waves, lane, kbuf[1]);
+    tree_stage_v(vb, first * kTreeStage, a.vstride, wave, waves, lane, vbuf[0]);
+    // What has been staged has landed when every wave has passed the barrier, and every wave is done with
+    // the other buffers. Stage st lies in buffer (st - first) % 2.
+    auto turn = [&](int st, int now) {
+      tree_landed();
+      __syncthreads();
+      if (st + 2 < end) tree_stage_k(kb, (st + 2) * kTreeStage, a.capacity, wave, waves, lane, kbuf[now]);
+      if (st + 1 < end) tree_stage_v(vb, (st + 1) * kTreeStage, a.vstride, wave, waves, lane, vbuf[now ^ 1]);
+    };
+    f32x16 s[2], next[2];
+    tree_scores(kbuf[0], t, col, hb, s);
+    int st = first;
+    for (; st + 2 <= clear; st += 2) {
+      turn(st, 0);
+      tree_step(kbuf[1], vbuf[0], t, s, next, col, hb);
+      turn(st + 1, 1);
+      tree_step(kbuf[0], vbuf[1], t, next, s, col, hb);  // behind the last stage, of what the buffer holds, and not used
+    }
+    for (; st < end; st++) {
+      const int now = (st - first) & 1;
+      turn(st, now);
+      if (care) {
+        for (int i = threadIdx.x; i < kTreeStage * 8; i += waves * kWave) {
+          v4u* v = reinterpret_cast<v4u*>(vbuf[now]) + i;
+          tree_clip(*v, st * kTreeStage + 8 * ((i & 7) ^ (i >> 4 & 7)), total, a.past);
+        }
+        __syncthreads();
+      }
+      tree_take(vbuf[now], t, s, col, hb, st * kTreeStage, a, mask);
+      if (st + 1 < end) tree_scores(kbuf[now ^ 1], t, col, hb, s);
+    }
+    if (!__syncthreads_or(mine && tree_odd(t.o)) || care) break;
+    tree_stage_k(kb, first * kTreeStage, a.capacity, wave, waves, lane, kbuf[0]);
   }
-  for (; st < end; st++) {
-    const int now = turn(st);
-    if (mine) tree_use<true>(buf[now], t, col, hb, st * kTreeStage, a, mask, vb);
+  if (!mine) return;
+  tree_store(a, part, part_ml, out_buf[wave], kvh, tile * kTreeCols, split, splits, lane, t.m, pair_sum(t.l), t.o);
+  if (care) {
+    tree_landed();  // the stores, which these overwrite
+    tree_add_odd(a, part, kvh, tile * kTreeCols, 0, 1, first * kTreeStage, min(end * kTreeStage, total), split, splits);
   }
-  t.l = pair_sum(t.l);
-  if (tile * kTreeCols + col < rows) tree_store(a, part, at, split, splits, hb, t.m, t.l, t.o);
 }
 
-// out[row] = the merge of its `splits` partials, a wave a row: lane (k, d) of 4 x 16 sums dimensions 4 d .. +3
-// over splits k, k + 4, ..., and the four sums are added in order.
-__global__ __launch_bounds__(kBlock) void k_attn_tree_merge(const float* __restrict__ part, float* __restrict__ out,
-                                                            int rows, int splits) {
-  const int lane = threadIdx.x & (kWave - 1), row = blockIdx.x * (kBlock / kWave) + threadIdx.x / kWave;
-  if (row >= rows) return;
-  const int k = lane >> 4, d = lane & 15;
-  const float* p = part + (size_t)row * splits * kTreePart;
+// The merge of a row's `splits` partials, a wave a row: lane (k, d) of 4 x 16 sums dimensions 4 d .. +3 over splits
+// k, k + 4, ..., and the four sums are added in order.
+__global__ __launch_bounds__(kBlock) void k_attn_tree_merge(TreeAttnArgs a, const float* __restrict__ part,
+                                                            const float* __restrict__ part_ml, int splits) {
+  const int lane = threadIdx.x & (kWave - 1), group = a.heads / a.kv_heads, rows = a.nodes * group;
+  const int at = blockIdx.x * (kBlock / kWave) + threadIdx.x / kWave;
+  if (at >= rows * a.kv_heads) return;
+  const int kvh = at / rows, row = at % rows, k = lane >> 4, d = lane & 15;
+  const size_t step = (size_t)a.kv_heads * rows;  // from split to split
+  const float* p = part + (size_t)at * kHeadDim + 4 * d;
+  const f32x2* ml = reinterpret_cast<const f32x2*>(part_ml) + at;
   float mx = -INFINITY;
-  for (int s = lane; s < splits; s += kWave) mx = fmaxf(mx, p[(size_t)s * kTreePart]);
+  for (int s = lane; s < splits; s += kWave) mx = fmaxf(mx, ml[s * step].x);
   mx = team_max<64>(mx);
   float l = 0.f;
   v4f o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int s = k; s < splits; s += 4) {
-    const float* ps = p + (size_t)s * kTreePart;
-    const float ms = ps[0], ls = ps[1];
-    const v4f x = *reinterpret_cast<const v4f*>(ps + 4 + 4 * d);
-    const float w = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - mx);
-    l = fmaf(w, ls, l);
+    const f32x2 w2 = ml[s * step];
+    const v4f x = *reinterpret_cast<const v4f*>(p + s * step * kHeadDim);
+    const float w = w2.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w2.x - mx);
+    l = fmaf(w, w2.y, l);
 #pragma unroll
     for (int r = 0; r < 4; r++) o[r] = fmaf(w, x[r], o[r]);
   }
@@ -525,31 +668,38 @@ __global__ __launch_bounds__(kBlock) void k_attn_tree_merge(const float* __restr
     o[r] += __shfl_xor(o[r], 32);
     o[r] = l == 0.f ? 0.f : o[r] / l;
   }
-  if (k == 0) *reinterpret_cast<v4f*>(out + (size_t)row * kHeadDim + 4 * d) = o;
+  if (k == 0) *reinterpret_cast<v4f*>(a.out + ((size_t)(row / group) * a.heads + kvh * group + row % group) * kHeadDim + 4 * d) = o;
 }
 
 namespace {
-// How a call is cut. `few`: waves take their keys from the cache themselves.
+// How a call is cut.
 struct TreePlan {
-  bool few;
-  int waves;   // many: column tiles of a block
+  bool direct;
+  int waves;   // staged: column tiles of a block
   int tiles;   // blocks along the rows
   int splits;  // ranges of keys
 };
 TreePlan tree_plan(int nodes, int past, int heads, int kv_heads) {
   TreePlan t;
   const int cols = (nodes * (heads / kv_heads) + kTreeCols - 1) / kTreeCols, total = past + nodes;
-  t.few = cols < 4;
-  t.tiles = t.few ? cols : (cols + kTreeWaves - 1) / kTreeWaves;
+  const int steps = (total + kTreeKeys - 1) / kTreeKeys, stages = (total + kTreeStage - 1) / kTreeStage;
+  t.direct = cols < 4 || steps <= 64;
+  if (t.direct) {
+    t.waves = 8;
+    t.tiles = cols;
+    t.splits = steps <= 64 ? 1 : std::max(1, std::min(std::min(256 / (t.tiles * kv_heads), kMaxTreeSplits), (steps + 7) / 8));
+    return t;
+  }
+  t.tiles = (cols + kTreeWaves - 1) / kTreeWaves;
   t.waves = (cols + t.tiles - 1) / t.tiles;
-  const int most = t.few ? (total + 4 * kTreeKeys - 1) / (4 * kTreeKeys) : (total + kTreeStage - 1) / kTreeStage;
-  int s = std::max(1, std::min(std::min(512 / (t.tiles * kv_heads), kMaxTreeSplits), most));
-  if (!t.few)
-    for (int e = s; e > s * 3 / 4; e--)
-      if (e * kv_heads % 8 == 0) {
-        s = e;
-        break;
-      }
+  // A range costs its share of about 1 us a stage; each one more, 0.14 us per 1000 rows written and merged.
+  const double want = sqrt(stages / (1.4e-4 * nodes * heads));
+  int s = std::max(1, std::min(std::min(256 / (t.tiles * kv_heads), kMaxTreeSplits), std::min(stages, (int)want)));
+  for (int e = s; e > s * 3 / 4; e--)
+    if (e * kv_heads % 8 == 0) {
+      s = e;
+      break;
+    }
   t.splits = s;
   return t;
 }
@@ -557,20 +707,21 @@ TreePlan tree_plan(int nodes, int past, int heads, int kv_heads) {
 
 size_t attention_tree_floats(int nodes, int past, int heads, int kv_heads) {
   const TreePlan t = tree_plan(nodes, past, heads, kv_heads);
-  return t.splits > 1 ? (size_t)nodes * heads * t.splits * kTreePart : 0;
+  return t.splits > 1 ? (size_t)nodes * heads * t.splits * (kHeadDim + 2) : 0;  // o, then (m, l)
 }
 
 hipError_t launch_attention_tree(hipStream_t s, const TreeAttnArgs& a, float* part) {
   const TreePlan t = tree_plan(a.nodes, a.past, a.heads, a.kv_heads);
-  if (t.few)
-    hipLaunchKernelGGL((k_attn_tree_few<1, 4>), dim3(t.splits, t.tiles, a.kv_heads), dim3(4 * kWave), 0, s, a, part);
+  float* ml = part + (size_t)a.nodes * a.heads * t.splits * kHeadDim;
+  if (t.direct)
+    hipLaunchKernelGGL((k_attn_tree_direct<8>), dim3(t.splits, t.tiles, a.kv_heads), dim3(8 * kWave), 0, s, a, part, ml);
   else
-    hipLaunchKernelGGL(k_attn_tree_many, dim3(t.splits * a.kv_heads * t.tiles), dim3(t.waves * kWave), 0, s, a, t.splits,
-                       t.tiles, part);
+    hipLaunchKernelGGL(k_attn_tree_staged, dim3(t.splits * a.kv_heads * t.tiles), dim3(t.waves * kWave), 0, s, a, t.splits,
+                       t.tiles, part, ml);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || t.splits == 1) return e;
   const int rows = a.nodes * a.heads;
-  hipLaunchKernelGGL(k_attn_tree_merge, dim3((rows + 3) / 4), dim3(kBlock), 0, s, part, a.out, rows, t.splits);
+  hipLaunchKernelGGL(k_attn_tree_merge, dim3((rows + 3) / 4), dim3(kBlock), 0, s, a, part, ml, t.splits);
   return hipGetLastError();
 }
 
