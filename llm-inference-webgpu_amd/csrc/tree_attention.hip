@@ -11,7 +11,7 @@
 //
 // Precision: K and V are exact in f16; q and p go in as two f16 terms each, sums are f32. A row's q is
 // first scaled by a power of two to below 2^14, so no finite q leaves f16's range and small ones keep
-// their bits; p is scaled by 2^15, so a weight of 2^-29 of the row's largest is still a normal f16 number.
+// their bits; p is scaled by 2^13, so a weight of 2^-27 of the row's largest is still a normal f16 number.
 //
 // Block: WQ x WK waves, WQ column tiles by WK runs of keys; wave (t, k) takes the 32-key steps k, k + WK, ...
 // of the block's range for column tile t, with an online softmax, and the WK states of a tile merge
@@ -28,7 +28,8 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int kTreeCols = 32;    // rows of a wave's tile
 constexpr int kTreeKeys = 32;    // keys of a step
 constexpr int kMaxTreeSplits = 128;
-constexpr float kWeightLog2 = 15.f;  // p is held as 2^15 p
+constexpr float kWeightLog2 = 13.f;  // p is held as 2^13 p of the running maximum's, which is
+constexpr float kMaxSlack = 2.f;     // left behind by up to 2^2: f16 holds up to 2^15
 
 // Where part k of n, even to one, of `count` begins.
 __host__ __device__ inline int tree_part(int count, int k, int n) { return (int)((int64_t)count * k / n); }
@@ -115,7 +116,8 @@ __device__ __forceinline__ float tree_query(const float* qr, f16x8 (&qh)[4], f16
   return __builtin_ldexpf(kScoreLog2, -up);
 }
 
-// The running maximum m of a row over N more scores, and l and o rescaled where it grew.
+// The reference m of a row's weights over N more scores: a maximum that may lag by kMaxSlack (in base-2 units), so
+// that l and o are seldom rescaled: a row's maximum grows by as much a few times in all.
 template <int N>
 __device__ __forceinline__ void tree_max(const f32x16 (&s)[N], float c, float& m, float& l, f32x16 (&o)[2]) {
   float big = s[0][0];
@@ -123,18 +125,20 @@ __device__ __forceinline__ void tree_max(const f32x16 (&s)[N], float c, float& m
   for (int j = 0; j < N; j++)
 #pragma unroll
     for (int i = 0; i < 16; i++) big = fmaxf(big, s[j][i]);
-  const float mn = fmaxf(m, pair_max(big) * c);
-  if (!__any(mn > m)) return;
-  const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+  const float mn = pair_max(big) * c;
+  const bool grow = mn > m + kMaxSlack;  // also from -inf
+  if (!__any(grow)) return;
+  const float to = grow ? mn : m;
+  const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - to);
   l *= alpha;
 #pragma unroll
   for (int dt = 0; dt < 2; dt++)
 #pragma unroll
     for (int i = 0; i < 16; i++) o[dt][i] *= alpha;
-  m = mn;
+  m = to;
 }
 
-// 32 scores of a row's pair of lanes to weights 2^15 2^(c s - m) in two f16 terms, their sum into l.
+// 32 scores of a row's pair of lanes to weights 2^13 2^(c s - m) in two f16 terms, their sum into l.
 __device__ __forceinline__ void tree_weights(const f32x16& s, float c, float m, float& l, f16x8 (&ph)[2], f16x8 (&pl)[2]) {
   const float shift = kWeightLog2 - (m == -INFINITY ? 0.f : m);
 #pragma unroll
@@ -420,20 +424,44 @@ constexpr int kTreeWaves = 8;
 // their own (vmcnt), so whoever reads them waits with tree_landed and meets the other waves. In asm, as the
 // compiler would have every later read of LDS wait for them, also one of another stage. `to` is
 // uniform; lane l's 16 bytes land at to + 16 l.
-__device__ __forceinline__ void copy_to_lds(const uint16_t* from, uint16_t* to) {
+__device__ __forceinline__ void copy_to_lds(const uint16_t* from, uint32_t offset, uint16_t* to) {
   const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)to);
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(offset), "s"(from) : "memory", "m0");
 }
-__device__ __forceinline__ void tree_stage_k(const uint16_t* kb, int p0, int capacity, int wave, int waves, int lane, uint16_t* buf) {
-  for (int j = wave; j < 8; j += waves) {
-    const int r = 8 * j + (lane >> 3), piece = (lane & 7) ^ (r >> 1 & 7);
-    copy_to_lds(kb + (size_t)min(p0 + (r & 32) + tree_key(r & 31), capacity - 1) * kHeadDim + 8 * piece, buf + j * 512);
+// A wave's share: rows 8 wave .. +7 of a stage, and 8 (wave + waves) .. where there are fewer waves than eight.
+struct TreeCopy {
+  const uint16_t *k, *v;    // uniform: the kv head's caches
+  uint32_t koff[2], voff;   // bytes of the lane's piece, from the stage's first key, from its rows' first dimension
+  int wave, waves, capacity, vstride, lane;
+};
+__device__ __forceinline__ TreeCopy tree_copy(const uint16_t* kb, const uint16_t* vb, int capacity, int vstride, int wave, int waves,
+                                              int lane) {
+  TreeCopy c{kb, vb, {0, 0}, 0, wave, waves, capacity, vstride, lane};
+  const int sub = lane >> 3;
+#pragma unroll
+  for (int t = 0; t < 2; t++) {
+    const int r = 8 * (wave + waves * t) + sub;
+    c.koff[t] = 128 * ((r & 32) + tree_key(r & 31)) + 16 * ((lane & 7) ^ (r >> 1 & 7));
+  }
+  c.voff = 2 * (uint32_t)vstride * sub;
+  return c;
+}
+__device__ __forceinline__ void tree_stage_k(const TreeCopy& c, int p0, uint16_t* buf) {
+#pragma unroll
+  for (int t = 0; t < 2; t++) {
+    const int j = c.wave + c.waves * t;
+    if (j >= 8) break;
+    uint32_t off = c.koff[t];
+    if (p0 + kTreeStage > c.capacity) off = min(off >> 7, (uint32_t)(c.capacity - 1 - p0)) << 7 | (off & 127);
+    copy_to_lds(c.k + (size_t)p0 * kHeadDim, off, buf + j * 512);
   }
 }
-__device__ __forceinline__ void tree_stage_v(const uint16_t* vb, int p0, int vstride, int wave, int waves, int lane, uint16_t* buf) {
-  for (int j = wave; j < 8; j += waves) {
-    const int r = 8 * j + (lane >> 3), piece = (lane & 7) ^ (r >> 1 & 7);
-    copy_to_lds(vb + (size_t)r * vstride + p0 + 8 * piece, buf + j * 512);
+__device__ __forceinline__ void tree_stage_v(const TreeCopy& c, int p0, uint16_t* buf) {
+#pragma unroll
+  for (int t = 0; t < 2; t++) {
+    const int j = c.wave + c.waves * t;
+    if (j >= 8) break;
+    copy_to_lds(c.v + (size_t)(8 * j) * c.vstride + p0, c.voff + (c.koff[t] & 127), buf + j * 512);
   }
 }
 __device__ __forceinline__ void tree_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
@@ -502,7 +530,7 @@ __device__ __forceinline__ void tree_take(const uint16_t* vbuf, TreeTile& t, f32
   }
 }
 
-// A stage in the past and the scores of the one after it, in one run of code without a branch, so that the
+// A stage in the past and the scores of the one after it, without a branch between them, so that the
 // matrix instructions of the scores run under the exponentials of the first half and those of the first
 // half's values under the second's.
 __device__ __forceinline__ void tree_step(const uint16_t* kbuf, const uint16_t* vbuf, TreeTile& t, const f32x16 (&s)[2],
@@ -512,19 +540,7 @@ __device__ __forceinline__ void tree_step(const uint16_t* kbuf, const uint16_t* 
   for (int ks = 0; ks < 4; ks++)
 #pragma unroll
     for (int j = 0; j < 2; j++) kf[ks][j] = __builtin_bit_cast(f16x8, tree_piece(kbuf, j, col, 2 * ks + hb));
-  float big = s[0][0];
-#pragma unroll
-  for (int j = 0; j < 2; j++)
-#pragma unroll
-    for (int i = 0; i < 16; i++) big = fmaxf(big, s[j][i]);
-  const float mn = fmaxf(t.m, pair_max(big) * t.c);
-  const float alpha = __builtin_amdgcn_exp2f(t.m - mn);  // 0 from -inf; the scores of the past are finite or NaN
-  t.m = mn;
-  t.l *= alpha;
-#pragma unroll
-  for (int dt = 0; dt < 2; dt++)
-#pragma unroll
-    for (int i = 0; i < 16; i++) t.o[dt][i] *= alpha;
+  tree_max(s, t.c, t.m, t.l, t.o);
 #pragma unroll
   for (int j = 0; j < 2; j++)
 #pragma unroll
@@ -578,7 +594,8 @@ __global__ __launch_bounds__(kWave * kTreeWaves, 2) void k_attn_tree_staged(Tree
   const int first = tree_part(stages, split, splits), end = tree_part(stages, split + 1, splits);
   const int clear = min(end, a.past / kTreeStage);  // the stages before it are all in the past
 
-  tree_stage_k(kb, first * kTreeStage, a.capacity, wave, waves, lane, kbuf[0]);
+  const TreeCopy copy = tree_copy(kb, vb, a.capacity, a.vstride, wave, waves, lane);
+  tree_stage_k(copy, first * kTreeStage, kbuf[0]);
   TreeTile t;
   t.c = tree_query(a.q + ((size_t)node * a.heads + head) * kHeadDim + 8 * hb, t.qh, t.ql);
   const bool mine = tile * kTreeCols < rows;
@@ -592,15 +609,15 @@ __global__ __launch_bounds__(kWave * kTreeWaves, 2) void k_attn_tree_staged(Tree
       for (int i = 0; i < 16; i++) t.o[dt][i] = 0.f;
     tree_landed();
     __syncthreads();
-    if (first + 1 < end) tree_stage_k(kb, (first + 1) * kTreeStage, a.capacity, wave, waves, lane, kbuf[1]);
-    tree_stage_v(vb, first * kTreeStage, a.vstride, wave, waves, lane, vbuf[0]);
+    if (first + 1 < end) tree_stage_k(copy, (first + 1) * kTreeStage, kbuf[1]);
+    tree_stage_v(copy, first * kTreeStage, vbuf[0]);
     // What has been staged has landed when every wave has passed the barrier, and every wave is done with
     // the other buffers. Stage st lies in buffer (st - first) % 2.
     auto turn = [&](int st, int now) {
       tree_landed();
       __syncthreads();
-      if (st + 2 < end) tree_stage_k(kb, (st + 2) * kTreeStage, a.capacity, wave, waves, lane, kbuf[now]);
-      if (st + 1 < end) tree_stage_v(vb, (st + 1) * kTreeStage, a.vstride, wave, waves, lane, vbuf[now ^ 1]);
+      if (st + 2 < end) tree_stage_k(copy, (st + 2) * kTreeStage, kbuf[now]);
+      if (st + 1 < end) tree_stage_v(copy, (st + 1) * kTreeStage, vbuf[now ^ 1]);
     };
     f32x16 s[2], next[2];
     tree_scores(kbuf[0], t, col, hb, s);
@@ -625,7 +642,7 @@ __global__ __launch_bounds__(kWave * kTreeWaves, 2) void k_attn_tree_staged(Tree
       if (st + 1 < end) tree_scores(kbuf[now ^ 1], t, col, hb, s);
     }
     if (!__syncthreads_or(mine && tree_odd(t.o)) || care) break;
-    tree_stage_k(kb, first * kTreeStage, a.capacity, wave, waves, lane, kbuf[0]);
+    tree_stage_k(copy, first * kTreeStage, kbuf[0]);
   }
   if (!mine) return;
   tree_store(a, part, part_ml, out_buf[wave], kvh, tile * kTreeCols, split, splits, lane, t.m, pair_sum(t.l), t.o);
