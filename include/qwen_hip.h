@@ -246,7 +246,8 @@ int qh_rope_append_tree(qh_ctx* ctx, const float* d_q, const float* d_k, const f
  * bits are allowed, those from `nodes` on are ignored). A node that sees nothing gets zeros. What a
  * node does not see has no influence on it, infinities and NaN included. q (rotated), out f32
  * [nodes, heads*64]; head h reads kv head h / (heads/kv_heads), any group; scale 1/8; head_dim must
- * be 64; buffers 16-byte aligned; nodes * heads at most 2^22. q.k and p.v on f16 MFMA with q and p in
+ * be 64; buffers 16-byte aligned; nodes * heads at most 2^22, capacity
+ * at most 2^27. q.k and p.v on f16 MFMA with q and p in
  * two f16 terms each, f32 sums (~1e-6 of the output). */
 int qh_attention_tree(qh_ctx* ctx, const float* d_q, const uint16_t* d_key_cache, const uint16_t* d_value_cache,
                       int32_t capacity, const uint64_t* d_mask, float* d_out, int32_t nodes, int32_t past,

@@ -666,6 +666,8 @@ int qh_attention_tree(qh_ctx* ctx, const float* d_q, const uint16_t* d_key_cache
   QH_CHECK(kv_heads >= 1 && heads >= kv_heads && heads % kv_heads == 0 && heads <= 65535, QH_ERR_INVALID,
            "heads %d / kv_heads %d must group evenly, at most 65535 heads", heads, kv_heads);
   QH_CHECK(nodes >= 1 && past >= 0, QH_ERR_INVALID, "attention_tree needs nodes >= 1 and past >= 0");
+  QH_CHECK(capacity <= 1 << 27, QH_ERR_INVALID, "attention_tree takes caches of up to 134217728 positions (capacity %d)",
+           capacity);
   QH_CHECK((int64_t)nodes * heads <= 1 << 22, QH_ERR_INVALID, "attention_tree takes at most 4194304 rows (%d nodes x %d heads)",
            nodes, heads);
   QH_CHECK((int64_t)past + nodes <= capacity, QH_ERR_RANGE, "attention over %lld positions exceeds capacity %d",

@@ -26,7 +26,6 @@ namespace qh {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int kTreeCols = 32;    // rows of a wave's tile
-constexpr int kTreeKeys = 32;    // keys of a step
 constexpr int kMaxTreeSplits = 128;
 constexpr float kWeightLog2 = 13.f;  // p is held as 2^13 p of the running maximum's, which is
 constexpr float kMaxSlack = 2.f;     // left behind by up to 2^2: f16 holds up to 2^15
@@ -52,20 +51,6 @@ __device__ __forceinline__ uint32_t tree_window(const uint64_t* mask, int words,
   return n < 32 ? win & ((1u << n) - 1u) : win;
 }
 
-__device__ __forceinline__ void tree_load_k(const uint16_t* kb, int p0, int capacity, int col, int hb, f16x8 (&k)[4]) {
-  const uint16_t* kr = kb + (size_t)min(p0 + tree_key(col), capacity - 1) * kHeadDim + 8 * hb;
-#pragma unroll
-  for (int ks = 0; ks < 4; ks++) k[ks] = *reinterpret_cast<const f16x8*>(kr + 16 * ks);
-}
-// p0 is a multiple of 32 below vstride, which is a multiple of 64.
-__device__ __forceinline__ void tree_load_v(const uint16_t* vb, int p0, int vstride, int col, int hb, v4u (&v)[2][2]) {
-#pragma unroll
-  for (int dt = 0; dt < 2; dt++)
-#pragma unroll
-    for (int ks = 0; ks < 2; ks++)
-      v[dt][ks] = *reinterpret_cast<const v4u*>(vb + (size_t)(32 * dt + col) * vstride + p0 + 16 * ks + 8 * hb);
-}
-
 // x and y of a row's two lanes (l, l + 32): their maximum, their sum.
 __device__ __forceinline__ float pair_max(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
@@ -87,18 +72,23 @@ __device__ __forceinline__ void f16_split(float x, float y, f16x2& hi, f16x2& lo
   lo = __builtin_convertvector((f32x2{dx, dy}), f16x2);
 }
 
-// The row's query (its 64 floats from qr + 8 hb) as B operands, and the factor of its scores.
-__device__ __forceinline__ float tree_query(const float* qr, f16x8 (&qh)[4], f16x8 (&ql)[4]) {
+// The row's query (its 64 floats from qr + 8 hb) as B operands, and the factor of its scores; the loads apart, as
+// a kernel has them before the keys', whose time the arithmetic then takes.
+struct TreeQuery {
   v4f x[4][2];
+};
+__device__ __forceinline__ void tree_load_query(const float* qr, TreeQuery& q) {
+#pragma unroll
+  for (int ks = 0; ks < 4; ks++)
+#pragma unroll
+    for (int e = 0; e < 2; e++) q.x[ks][e] = *reinterpret_cast<const v4f*>(qr + 16 * ks + 4 * e);
+}
+__device__ __forceinline__ float tree_query(const TreeQuery& q, f16x8 (&qh)[4], f16x8 (&ql)[4]) {
   float big = 0.f;
 #pragma unroll
   for (int ks = 0; ks < 4; ks++)
 #pragma unroll
-    for (int e = 0; e < 2; e++) {
-      x[ks][e] = *reinterpret_cast<const v4f*>(qr + 16 * ks + 4 * e);
-#pragma unroll
-      for (int r = 0; r < 4; r++) big = fmaxf(big, fabsf(x[ks][e][r]));
-    }
+    for (int e = 0; e < 8; e++) big = fmaxf(big, fabsf(q.x[ks][e / 4][e % 4]));
   big = pair_max(big);
   const int up = big > 0.f && big < INFINITY ? min(14 - __builtin_amdgcn_frexp_expf(big), 100) : 0;
 #pragma unroll
@@ -106,8 +96,8 @@ __device__ __forceinline__ float tree_query(const float* qr, f16x8 (&qh)[4], f16
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
       f16x2 hi, lo;
-      f16_split(f32_pinned(__builtin_ldexpf(x[ks][e / 4][e % 4], up)), f32_pinned(__builtin_ldexpf(x[ks][e / 4][e % 4 + 1], up)),
-                hi, lo);
+      f16_split(f32_pinned(__builtin_ldexpf(q.x[ks][e / 4][e % 4], up)),
+                f32_pinned(__builtin_ldexpf(q.x[ks][e / 4][e % 4 + 1], up)), hi, lo);
       qh[ks][e] = hi.x;
       qh[ks][e + 1] = hi.y;
       ql[ks][e] = lo.x;
@@ -254,217 +244,30 @@ __device__ __forceinline__ void tree_store(const TreeAttnArgs& a, float* part, f
   }
 }
 
-// Short contexts and few rows: each wave takes its keys straight from the cache. A block of WK waves has a
-// tile of rows and a range of keys; wave w takes the 32-key steps w, w + WK, ... of it, the next step's
-// loads in flight, and the waves' states merge through LDS, each wave merging its share of the dimensions
-// over all of them in order.
-template <int WK>
-__global__ __launch_bounds__(kWave * WK, 2) void k_attn_tree_direct(TreeAttnArgs a, float* __restrict__ part, float* __restrict__ part_ml) {
-  constexpr int kGroups = 8;  // of four dimensions: 32 (g / 4) + 8 (g % 4) + 4 hb .. +3
-  __shared__ v4f sh_o[WK][kGroups][kWave];
-  __shared__ float sh_m[WK][kTreeCols], sh_l[WK][kTreeCols];
-  const int lane = threadIdx.x & (kWave - 1), wk = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int col = lane & 31, hb = lane >> 5;
-  const int group = a.heads / a.kv_heads, rows = a.nodes * group;
-  const int kvh = blockIdx.z, total = a.past + a.nodes, words = (a.nodes + 63) / 64;
-  const int row = min((int)blockIdx.y * kTreeCols + col, rows - 1);  // past the end, a copy of the last
-  const int node = row / group, head = kvh * group + row % group;
-  const uint16_t* kb = a.kc + (size_t)kvh * a.capacity * kHeadDim;
-  const uint16_t* vb = a.vt + (size_t)kvh * kHeadDim * a.vstride;
-  const uint64_t* mask = a.mask + (size_t)node * words;
-  const int steps = (total + kTreeKeys - 1) / kTreeKeys;
-  const int first = tree_part(steps, blockIdx.x, gridDim.x) + wk, end = tree_part(steps, blockIdx.x + 1, gridDim.x);
+// Keys come through LDS in stages of 32 H: K rows of 128 bytes in tree_key's order, V rows of 64 H bytes, a
+// dimension's keys. Their 16-byte pieces are stored at piece ^ (row / 2 % 8), or ^ (row / 4 % 4) in rows of 64 bytes, so
+// that the 16 lanes of a read's cycle, which want one piece of 16 rows, find it in different banks. (Operands
+// loaded straight from the caches, 32 bytes of 32 lines an instruction, kept a CU's cache busy for 3000-4000 cycles per
+// 32 keys of eight waves.)
 
-  f16x8 kf[4];
-  v4u vf[2][2];
-  uint32_t win, next_win = 0xffffffffu;
-  auto look = [&](int step) {
-    const int p0 = step * kTreeKeys;
-    next_win = p0 + kTreeKeys > a.past ? tree_window(mask, words, a.nodes, a.past, p0) : 0xffffffffu;
-  };
-  if (first < end) {
-    tree_load_k(kb, first * kTreeKeys, a.capacity, col, hb, kf);
-    tree_load_v(vb, first * kTreeKeys, a.vstride, col, hb, vf);
-    look(first);
-  }
-  f16x8 qh[4], ql[4];
-  const size_t at = (size_t)node * a.heads + head;
-  const float c = tree_query(a.q + at * kHeadDim + 8 * hb, qh, ql);
-  __shared__ float sh_out[kTreeCols][kStoreRow];
-  float m, l, mx;
-  bool care = false;
-  for (;; care = true) {
-    m = -INFINITY;
-    l = 0.f;
-    f32x16 o[2];
-#pragma unroll
-    for (int dt = 0; dt < 2; dt++)
-#pragma unroll
-      for (int i = 0; i < 16; i++) o[dt][i] = 0.f;
-    for (int step = first; step < end; step += WK) {
-      const int p0 = step * kTreeKeys;
-      const bool more = step + WK < end;
-      f32x16 s[1];
-#pragma unroll
-      for (int i = 0; i < 16; i++) s[0][i] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < 4; ks++) s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[ks], qh[ks], s[0], 0, 0, 0);
-#pragma unroll
-      for (int ks = 0; ks < 4; ks++) s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[ks], ql[ks], s[0], 0, 0, 0);
-      win = next_win;
-      if (more) {
-        tree_load_k(kb, p0 + WK * kTreeKeys, a.capacity, col, hb, kf);
-        look(step + WK);
-      }
-      if (p0 + kTreeKeys > a.past) tree_hide(s[0], win, hb);  // uniform
-      tree_max(s, c, m, l, o);
-      f16x8 ph[2], pl[2];
-      tree_weights(s[0], c, m, l, ph, pl);
-      if (p0 + kTreeKeys > total) {
-#pragma unroll
-        for (int dt = 0; dt < 2; dt++)
-#pragma unroll
-          for (int ks = 0; ks < 2; ks++) tree_clip(vf[dt][ks], p0 + 16 * ks + 8 * hb, total);
-      }
-      if (care) {
-#pragma unroll
-        for (int dt = 0; dt < 2; dt++)
-#pragma unroll
-          for (int ks = 0; ks < 2; ks++) tree_clip(vf[dt][ks], p0 + 16 * ks + 8 * hb, total, a.past);
-      }
-#pragma unroll
-      for (int ks = 0; ks < 2; ks++) {
-#pragma unroll
-        for (int dt = 0; dt < 2; dt++)
-          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, vf[dt][ks]), ph[ks], o[dt], 0, 0, 0);
-#pragma unroll
-        for (int dt = 0; dt < 2; dt++)
-          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, vf[dt][ks]), pl[ks], o[dt], 0, 0, 0);
-      }
-      if (more) tree_load_v(vb, p0 + WK * kTreeKeys, a.vstride, col, hb, vf);
-    }
-    l = pair_sum(l);
-
-#pragma unroll
-    for (int g = 0; g < kGroups; g++) {
-      const int dt = g / 4, i = 4 * (g % 4);
-      sh_o[wk][g][lane] = v4f{o[dt][i], o[dt][i + 1], o[dt][i + 2], o[dt][i + 3]};
-    }
-    if (hb == 0) {
-      sh_m[wk][col] = m;
-      sh_l[wk][col] = l;
-    }
-    __syncthreads();
-    // Each wave merges its share of the dimensions; the tile's rows leave through LDS.
-    float wt[WK];
-    mx = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < WK; w++) {
-      wt[w] = sh_m[w][col];
-      mx = fmaxf(mx, wt[w]);
-    }
-    l = 0.f;
-#pragma unroll
-    for (int w = 0; w < WK; w++) {
-      wt[w] = wt[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(wt[w] - mx);
-      l = fmaf(sh_l[w][col], wt[w], l);
-    }
-    const float scale = gridDim.x > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-    float z = 0.f;
-#pragma unroll
-    for (int k = 0; k < kGroups / WK; k++) {
-      const int g = wk * (kGroups / WK) + k;
-      v4f x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int w = 0; w < WK; w++) {
-        const v4f y = sh_o[w][g][lane];
-#pragma unroll
-        for (int r = 0; r < 4; r++) x[r] = fmaf(y[r], wt[w], x[r]);
-      }
-#pragma unroll
-      for (int r = 0; r < 4; r++) {
-        z = fmaf(x[r], 0.f, z);
-        x[r] *= scale;
-      }
-      *reinterpret_cast<v4f*>(&sh_out[col][32 * (g / 4) + 8 * (g % 4) + 4 * hb]) = x;
-    }
-    if (!__syncthreads_or(z != 0.f) || care) break;
-    if (first < end) {
-      tree_load_k(kb, first * kTreeKeys, a.capacity, col, hb, kf);
-      tree_load_v(vb, first * kTreeKeys, a.vstride, col, hb, vf);
-      look(first);
-    }
-  }
-  const int row0 = blockIdx.y * kTreeCols;
-  const size_t slot = tree_slot(kvh, rows, row0, a.kv_heads, blockIdx.x);
-  if (gridDim.x > 1 && wk == 0 && hb == 0 && row0 + col < rows) *reinterpret_cast<f32x2*>(part_ml + 2 * (slot + col)) = f32x2{mx, l};
-  for (int i = threadIdx.x; i < kTreeCols * 16; i += kWave * WK) {
-    const int r = i >> 4;
-    if (row0 + r >= rows) break;
-    float* dst = gridDim.x > 1 ? part + (slot + r) * kHeadDim
-                               : a.out + ((size_t)((row0 + r) / group) * a.heads + kvh * group + (row0 + r) % group) * kHeadDim;
-    *reinterpret_cast<v4f*>(dst + 4 * (i & 15)) = *reinterpret_cast<const v4f*>(&sh_out[r][4 * (i & 15)]);
-  }
-  if (care) {
-    __syncthreads();
-    tree_add_odd(a, part, kvh, row0, wk, WK, kTreeKeys * tree_part(steps, blockIdx.x, gridDim.x), min(kTreeKeys * end, total), blockIdx.x,
-                 gridDim.x);
-  }
-}
-
-// Long contexts and many rows: a block's waves, a column tile each, share stages of 64 keys (whole 128-byte
-// lines of both caches) in LDS. LDS rows are 128 bytes, K's in tree_key's order; their 16-byte pieces are stored
-// at piece ^ (row / 2 % 8), so that the 16 lanes of a read's cycle, which want one piece of 16 rows, find it in
-// different banks. A stage's scores are made while the weights of the one before it are: its K is
-// staged one turn ahead of its V, and the products' matrix instructions have the exponentials to run under.
-constexpr int kTreeStage = 64;
-constexpr int kTreeWaves = 8;
-
-// The copies of one stage of K or V, 8 of 1 KB (8 rows each, 16 bytes a lane), dealt to the waves. They land on
-// their own (vmcnt), so whoever reads them waits with tree_landed and meets the other waves. In asm, as the
-// compiler would have every later read of LDS wait for them, also one of another stage. `to` is
-// uniform; lane l's 16 bytes land at to + 16 l.
+// 64 lanes' 16 bytes at from + offset to LDS, lane l's to `to` + 16 l (`from` and `to` uniform). It lands on its own
+// (vmcnt): whoever reads it waits with tree_landed. In asm, as the compiler would have every later read of LDS wait for
+// it, also one of another stage.
 __device__ __forceinline__ void copy_to_lds(const uint16_t* from, uint32_t offset, uint16_t* to) {
   const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)to);
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(offset), "s"(from) : "memory", "m0");
 }
-// A wave's share: rows 8 wave .. +7 of a stage, and 8 (wave + waves) .. where there are fewer waves than eight.
-struct TreeCopy {
-  const uint16_t *k, *v;    // uniform: the kv head's caches
-  uint32_t koff[2], voff;   // bytes of the lane's piece, from the stage's first key, from its rows' first dimension
-  int wave, waves, capacity, vstride, lane;
-};
-__device__ __forceinline__ TreeCopy tree_copy(const uint16_t* kb, const uint16_t* vb, int capacity, int vstride, int wave, int waves,
-                                              int lane) {
-  TreeCopy c{kb, vb, {0, 0}, 0, wave, waves, capacity, vstride, lane};
-  const int sub = lane >> 3;
-#pragma unroll
-  for (int t = 0; t < 2; t++) {
-    const int r = 8 * (wave + waves * t) + sub;
-    c.koff[t] = 128 * ((r & 32) + tree_key(r & 31)) + 16 * ((lane & 7) ^ (r >> 1 & 7));
-  }
-  c.voff = 2 * (uint32_t)vstride * sub;
-  return c;
+// Until at most N of the wave's copies and loads are still on their way.
+template <int N>
+__device__ __forceinline__ void tree_landed() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ void tree_stage_k(const TreeCopy& c, int p0, uint16_t* buf) {
-#pragma unroll
-  for (int t = 0; t < 2; t++) {
-    const int j = c.wave + c.waves * t;
-    if (j >= 8) break;
-    uint32_t off = c.koff[t];
-    if (p0 + kTreeStage > c.capacity) off = min(off >> 7, (uint32_t)(c.capacity - 1 - p0)) << 7 | (off & 127);
-    copy_to_lds(c.k + (size_t)p0 * kHeadDim, off, buf + j * 512);
-  }
+// A lane's share of copy j (0 .. 7) of a stage's K, LDS rows 8 j .. +7: its key in the stage and bytes into its row.
+__device__ __forceinline__ uint32_t copy_key(int j, int lane) {
+  const int r = 8 * j + (lane >> 3);
+  return (r & 32) + tree_key(r & 31);
 }
-__device__ __forceinline__ void tree_stage_v(const TreeCopy& c, int p0, uint16_t* buf) {
-#pragma unroll
-  for (int t = 0; t < 2; t++) {
-    const int j = c.wave + c.waves * t;
-    if (j >= 8) break;
-    copy_to_lds(c.v + (size_t)(8 * j) * c.vstride + p0, c.voff + (c.koff[t] & 127), buf + j * 512);
-  }
-}
-__device__ __forceinline__ void tree_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ uint32_t copy_piece(int j, int lane) { return 16 * ((lane & 7) ^ (4 * (j & 1) + (lane >> 4))); }
 
 // What a wave keeps of its tile of rows.
 struct TreeTile {
@@ -472,44 +275,72 @@ struct TreeTile {
   float c, m, l;
   f32x16 o[2];
 };
-
-// The operand of 16-byte piece `piece` of LDS row 32 half + col.
-__device__ __forceinline__ v4u tree_piece(const uint16_t* buf, int half, int col, int piece) {
-  return *reinterpret_cast<const v4u*>(buf + (32 * half + col) * kTreeStage + 8 * (piece ^ (col >> 1 & 7)));
+__device__ __forceinline__ void tree_begin(TreeTile& t) {
+  t.m = -INFINITY;
+  t.l = 0.f;
+#pragma unroll
+  for (int dt = 0; dt < 2; dt++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) t.o[dt][i] = 0.f;
 }
 
-__device__ __forceinline__ void tree_scores(const uint16_t* kbuf, const TreeTile& t, int col, int hb, f32x16 (&s)[2]) {
+// 16-byte piece `piece` of a K row, of a V row.
+__device__ __forceinline__ f16x8 tree_k(const uint16_t* kbuf, int row, int piece) {
+  return *reinterpret_cast<const f16x8*>(kbuf + row * kHeadDim + 8 * (piece ^ (row >> 1 & 7)));
+}
+template <int H>
+__device__ __forceinline__ int tree_v_at(int dim, int piece) {
+  return dim * 32 * H + 8 * (piece ^ (H == 2 ? dim >> 1 & 7 : dim >> 2 & 3));
+}
+template <int H>
+__device__ __forceinline__ v4u tree_v(const uint16_t* vbuf, int dim, int piece) {
+  return *reinterpret_cast<const v4u*>(vbuf + tree_v_at<H>(dim, piece));
+}
+
+// With care (tree_odd): a stage's V without the infinite and NaN values of nodes, in place; threads `first`, + `threads`, ...
+template <int H>
+__device__ __forceinline__ void tree_clean(uint16_t* vbuf, int p0, int total, int past, int first, int threads) {
+  for (int i = first; i < kHeadDim * 4 * H; i += threads) {
+    const int dim = i / (4 * H), piece = i % (4 * H);
+    tree_clip(*reinterpret_cast<v4u*>(vbuf + tree_v_at<H>(dim, piece)), p0 + 8 * piece, total, past);
+  }
+}
+
+template <int H>
+__device__ __forceinline__ void tree_scores(const uint16_t* kbuf, const TreeTile& t, int col, int hb, f32x16 (&s)[H]) {
 #pragma unroll
-  for (int j = 0; j < 2; j++)
+  for (int j = 0; j < H; j++)
 #pragma unroll
     for (int i = 0; i < 16; i++) s[j][i] = 0.f;
 #pragma unroll
   for (int ks = 0; ks < 4; ks++) {
-    f16x8 kf[2];
+    f16x8 kf[H];
 #pragma unroll
-    for (int j = 0; j < 2; j++) kf[j] = __builtin_bit_cast(f16x8, tree_piece(kbuf, j, col, 2 * ks + hb));
+    for (int j = 0; j < H; j++) kf[j] = tree_k(kbuf, 32 * j + col, 2 * ks + hb);
 #pragma unroll
-    for (int j = 0; j < 2; j++) s[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[j], t.qh[ks], s[j], 0, 0, 0);
+    for (int j = 0; j < H; j++) s[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[j], t.qh[ks], s[j], 0, 0, 0);
 #pragma unroll
-    for (int j = 0; j < 2; j++) s[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[j], t.ql[ks], s[j], 0, 0, 0);
+    for (int j = 0; j < H; j++) s[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[j], t.ql[ks], s[j], 0, 0, 0);
   }
 }
 
-// The stage of scores s into the tile's state, where some of its keys may be nodes or lie behind the last one.
-__device__ __forceinline__ void tree_take(const uint16_t* vbuf, TreeTile& t, f32x16 (&s)[2], int col, int hb, int p0,
-                                          const TreeAttnArgs& a, const uint64_t* mask) {
+// What the lane's row sees of positions p0 .. p0+31, wherever they lie.
+__device__ __forceinline__ uint32_t tree_sees(const TreeAttnArgs& a, const uint64_t* mask, int p0) {
+  return p0 + 32 <= a.past ? 0xffffffffu : p0 < a.past + a.nodes ? tree_window(mask, (a.nodes + 63) / 64, a.nodes, a.past, p0) : 0u;
+}
+
+// The stage of scores s at p0 into the tile's state; win: what the row sees of it, where some of its keys may be nodes.
+template <int H>
+__device__ __forceinline__ void tree_take(const uint16_t* vbuf, TreeTile& t, f32x16 (&s)[H], int col, int hb, int p0,
+                                          const TreeAttnArgs& a, const uint32_t (&win)[H]) {
   const int total = a.past + a.nodes;
-  {
+  if (p0 + 32 * H > a.past) {  // uniform
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
-      const int q0 = p0 + 32 * j;
-      const uint32_t win = q0 + 32 <= a.past ? 0xffffffffu : q0 < total ? tree_window(mask, (a.nodes + 63) / 64, a.nodes, a.past, q0) : 0u;
-      tree_hide(s[j], win, hb);
-    }
+    for (int j = 0; j < H; j++) tree_hide(s[j], win[j], hb);
   }
   tree_max(s, t.c, t.m, t.l, t.o);
 #pragma unroll
-  for (int j = 0; j < 2; j++) {
+  for (int j = 0; j < H; j++) {
     f16x8 ph[2], pl[2];
     tree_weights(s[j], t.c, t.m, t.l, ph, pl);
 #pragma unroll
@@ -517,8 +348,8 @@ __device__ __forceinline__ void tree_take(const uint16_t* vbuf, TreeTile& t, f32
       v4u v[2];
 #pragma unroll
       for (int dt = 0; dt < 2; dt++) {
-        v[dt] = tree_piece(vbuf, dt, col, 4 * j + 2 * ks + hb);
-        tree_clip(v[dt], p0 + 32 * j + 16 * ks + 8 * hb, total);
+        v[dt] = tree_v<H>(vbuf, 32 * dt + col, 4 * j + 2 * ks + hb);
+        if (p0 + 32 * H > total) tree_clip(v[dt], p0 + 32 * j + 16 * ks + 8 * hb, total);
       }
 #pragma unroll
       for (int dt = 0; dt < 2; dt++)
@@ -530,6 +361,147 @@ __device__ __forceinline__ void tree_take(const uint16_t* vbuf, TreeTile& t, f32
   }
 }
 
+// Short contexts and few rows: a block of WK waves has a tile of rows and a range of keys, and wave w takes the
+// 32-key stages w, w + WK, ... of it in two buffers of its own, the next one on its way. The waves' states merge through LDS, each wave merging its share of the dimensions over
+// all of them in order.
+template <int WK>
+__global__ __launch_bounds__(kWave * WK, 2) void k_attn_tree_direct(TreeAttnArgs a, float* __restrict__ part,
+                                                                  float* __restrict__ part_ml) {
+  constexpr int kGroups = 8;  // of four dimensions: 32 (g / 4) + 8 (g % 4) + 4 hb .. +3
+  constexpr int kStage = 32, kStageSize = kStage * kHeadDim;
+  union Shared {
+    uint16_t stage[WK][2][2][kStageSize];  // K and V, twice
+    struct {
+      v4f o[WK][kGroups][kWave];
+      float m[WK][kTreeCols], l[WK][kTreeCols], out[kTreeCols][kStoreRow];
+    } end;
+  };
+  __shared__ __attribute__((aligned(16))) Shared sh;
+  const int lane = threadIdx.x & (kWave - 1), wk = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int col = lane & 31, hb = lane >> 5;
+  const int group = a.heads / a.kv_heads, rows = a.nodes * group;
+  const int kvh = blockIdx.z, total = a.past + a.nodes;
+  const int row0 = blockIdx.y * kTreeCols, row = min(row0 + col, rows - 1);  // past the end, a copy of the last
+  const int node = row / group;
+  const size_t at = (size_t)node * a.heads + kvh * group + row % group;
+  const uint64_t* mask = a.mask + (size_t)node * ((a.nodes + 63) / 64);
+  const int stages = (total + kStage - 1) / kStage;
+  const int begin = tree_part(stages, blockIdx.x, gridDim.x), end = tree_part(stages, blockIdx.x + 1, gridDim.x);
+  const int first = begin + wk;
+
+  TreeQuery query;
+  tree_load_query(a.q + at * kHeadDim + 8 * hb, query);
+  const uint16_t* kb = a.kc + (size_t)kvh * a.capacity * kHeadDim;
+  const uint16_t* vb = a.vt + (size_t)kvh * kHeadDim * a.vstride;
+  // K rows 8 j .. +7 of copy j, V dimensions 16 j .. +15: eight copies a stage.
+  const uint32_t voff = 2 * (uint32_t)a.vstride * (lane >> 2) + 16 * ((lane & 3) ^ (lane >> 4));
+  auto copy = [&](int st, uint16_t (&buf)[2][kStageSize]) {
+    const int p0 = st * kStage;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const uint32_t key = min(copy_key(j, lane), (uint32_t)(a.capacity - 1 - p0));
+      copy_to_lds(kb + (size_t)p0 * kHeadDim, 128 * key + copy_piece(j, lane), buf[0] + j * 512);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) copy_to_lds(vb + (size_t)(16 * j) * a.vstride + p0, voff, buf[1] + j * 512);
+  };
+  if (first < end) copy(first, sh.stage[wk][0]);
+  TreeTile t;
+  t.c = tree_query(query, t.qh, t.ql);
+  float mx;
+  bool care = false;
+  for (;; care = true) {
+    tree_begin(t);
+    int turn = 0;
+    for (int st = first; st < end; st += WK, turn ^= 1) {
+      const int p0 = st * kStage;
+      uint32_t win[1] = {0xffffffffu};
+      if (p0 + kStage > a.past) win[0] = tree_sees(a, mask, p0);
+      uint16_t(&buf)[2][kStageSize] = sh.stage[wk][turn];
+      if (st + WK < end) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the other buffer has been read
+        copy(st + WK, sh.stage[wk][turn ^ 1]);
+        tree_landed<8>();  // all but those
+      } else {
+        tree_landed<0>();
+      }
+      f32x16 s[1];
+      tree_scores(buf[0], t, col, hb, s);
+      if (care) {
+        tree_clean<1>(buf[1], p0, total, a.past, lane, kWave);
+        wave_lds_handoff();
+      }
+      tree_take(buf[1], t, s, col, hb, p0, a, win);
+    }
+    t.l = pair_sum(t.l);
+    __syncthreads();  // the stages' LDS is free
+#pragma unroll
+    for (int g = 0; g < kGroups; g++) {
+      const int dt = g / 4, i = 4 * (g % 4);
+      sh.end.o[wk][g][lane] = v4f{t.o[dt][i], t.o[dt][i + 1], t.o[dt][i + 2], t.o[dt][i + 3]};
+    }
+    if (hb == 0) {
+      sh.end.m[wk][col] = t.m;
+      sh.end.l[wk][col] = t.l;
+    }
+    __syncthreads();
+    // Each wave merges its share of the dimensions; the tile's rows leave through LDS.
+    float wt[WK];
+    mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WK; w++) {
+      wt[w] = sh.end.m[w][col];
+      mx = fmaxf(mx, wt[w]);
+    }
+    t.l = 0.f;
+#pragma unroll
+    for (int w = 0; w < WK; w++) {
+      wt[w] = wt[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(wt[w] - mx);
+      t.l = fmaf(sh.end.l[w][col], wt[w], t.l);
+    }
+    const float scale = gridDim.x > 1 ? 1.f : t.l == 0.f ? 0.f : 1.f / t.l;
+    float z = 0.f;
+#pragma unroll
+    for (int k = 0; k < kGroups / WK; k++) {
+      const int g = wk * (kGroups / WK) + k;
+      v4f x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < WK; w++) {
+        const v4f y = sh.end.o[w][g][lane];
+#pragma unroll
+        for (int r = 0; r < 4; r++) x[r] = fmaf(y[r], wt[w], x[r]);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        z = fmaf(x[r], 0.f, z);
+        x[r] *= scale;
+      }
+      *reinterpret_cast<v4f*>(&sh.end.out[col][32 * (g / 4) + 8 * (g % 4) + 4 * hb]) = x;
+    }
+    if (!__syncthreads_or(z != 0.f) || care) break;
+    if (first < end) copy(first, sh.stage[wk][0]);
+  }
+  const size_t slot = tree_slot(kvh, rows, row0, a.kv_heads, blockIdx.x);
+  if (gridDim.x > 1 && wk == 0 && hb == 0 && row0 + col < rows) *reinterpret_cast<f32x2*>(part_ml + 2 * (slot + col)) = f32x2{mx, t.l};
+  for (int i = threadIdx.x; i < kTreeCols * 16; i += kWave * WK) {
+    const int r = i >> 4;
+    if (row0 + r >= rows) break;
+    float* dst = gridDim.x > 1 ? part + (slot + r) * kHeadDim
+                               : a.out + ((size_t)((row0 + r) / group) * a.heads + kvh * group + (row0 + r) % group) * kHeadDim;
+    *reinterpret_cast<v4f*>(dst + 4 * (i & 15)) = *reinterpret_cast<const v4f*>(&sh.end.out[r][4 * (i & 15)]);
+  }
+  if (care) {
+    __syncthreads();
+    tree_add_odd(a, part, kvh, row0, wk, WK, begin * kStage, min(end * kStage, total), blockIdx.x, gridDim.x);
+  }
+}
+
+// Long contexts and many rows: a block's waves, a column tile each, share the stages. A stage's scores are made while
+// the weights of the one before it are: its K is copied one turn ahead of its V, and the products' matrix
+// instructions have the exponentials to run under.
+constexpr int kTreeStage = 64;
+constexpr int kTreeWaves = 8;
+
 // A stage in the past and the scores of the one after it, without a branch between them, so that the
 // matrix instructions of the scores run under the exponentials of the first half and those of the first
 // half's values under the second's.
@@ -539,7 +511,7 @@ __device__ __forceinline__ void tree_step(const uint16_t* kbuf, const uint16_t* 
 #pragma unroll
   for (int ks = 0; ks < 4; ks++)
 #pragma unroll
-    for (int j = 0; j < 2; j++) kf[ks][j] = __builtin_bit_cast(f16x8, tree_piece(kbuf, j, col, 2 * ks + hb));
+    for (int j = 0; j < 2; j++) kf[ks][j] = tree_k(kbuf, 32 * j + col, 2 * ks + hb);
   tree_max(s, t.c, t.m, t.l, t.o);
 #pragma unroll
   for (int j = 0; j < 2; j++)
@@ -560,7 +532,7 @@ __device__ __forceinline__ void tree_step(const uint16_t* kbuf, const uint16_t* 
     for (int ks = 0; ks < 2; ks++) {
       v4u v[2];
 #pragma unroll
-      for (int dt = 0; dt < 2; dt++) v[dt] = tree_piece(vbuf, dt, col, 4 * j + 2 * ks + hb);
+      for (int dt = 0; dt < 2; dt++) v[dt] = tree_v<2>(vbuf, 32 * dt + col, 4 * j + 2 * ks + hb);
 #pragma unroll
       for (int dt = 0; dt < 2; dt++)
         t.o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, v[dt]), ph[ks], t.o[dt], 0, 0, 0);
@@ -583,71 +555,91 @@ __global__ __launch_bounds__(kWave * kTreeWaves, 2) void k_attn_tree_staged(Tree
   const int range = ranges % 8 ? b % ranges : (b & 7) + 8 * ((b >> 3) / tiles);
   const int split = range % splits, kvh = range / splits;
   const int group = a.heads / a.kv_heads, rows = a.nodes * group;
-  const int total = a.past + a.nodes, words = (a.nodes + 63) / 64;
+  const int total = a.past + a.nodes;
   const int tile = (ranges % 8 ? b / ranges : (b >> 3) % tiles) * waves + wave;
   const int row = min(tile * kTreeCols + col, rows - 1);  // past the end, a copy of the last
   const int node = row / group, head = kvh * group + row % group;
-  const uint16_t* kb = a.kc + (size_t)kvh * a.capacity * kHeadDim;
-  const uint16_t* vb = a.vt + (size_t)kvh * kHeadDim * a.vstride;
-  const uint64_t* mask = a.mask + (size_t)node * words;
+  const uint64_t* mask = a.mask + (size_t)node * ((a.nodes + 63) / 64);
   const int stages = (total + kTreeStage - 1) / kTreeStage;
   const int first = tree_part(stages, split, splits), end = tree_part(stages, split + 1, splits);
   const int clear = min(end, a.past / kTreeStage);  // the stages before it are all in the past
 
-  const TreeCopy copy = tree_copy(kb, vb, a.capacity, a.vstride, wave, waves, lane);
-  tree_stage_k(copy, first * kTreeStage, kbuf[0]);
+  TreeQuery query;
+  tree_load_query(a.q + ((size_t)node * a.heads + head) * kHeadDim + 8 * hb, query);
+  // The eight copies of a stage's K (rows 8 j .. +7) or V (dimensions 8 j .. +7), dealt to the waves: one or two each.
+  const uint16_t* kb = a.kc + (size_t)kvh * a.capacity * kHeadDim;
+  const uint16_t* vb[2];
+  uint32_t koff[2], voff[2];
+#pragma unroll
+  for (int e = 0; e < 2; e++) {
+    const int j = (wave + waves * e) & 7;
+    koff[e] = 128 * copy_key(j, lane) + copy_piece(j, lane);
+    vb[e] = a.vt + ((size_t)kvh * kHeadDim + 8 * j) * a.vstride;
+    voff[e] = 2 * (uint32_t)a.vstride * (lane >> 3) + copy_piece(j, lane);
+  }
+  const bool two = wave + waves < 8;
+  auto copy_k = [&](int st) {
+    const int p0 = st * kTreeStage;
+    uint16_t* to = kbuf[(st - first) & 1] + wave * 512;
+    uint32_t off[2] = {koff[0], koff[1]};
+    if (p0 + kTreeStage > a.capacity) {
+#pragma unroll
+      for (int e = 0; e < 2; e++) off[e] = min(off[e] >> 7, (uint32_t)(a.capacity - 1 - p0)) << 7 | (off[e] & 127);
+    }
+    copy_to_lds(kb + (size_t)p0 * kHeadDim, off[0], to);
+    if (two) copy_to_lds(kb + (size_t)p0 * kHeadDim, off[1], to + waves * 512);
+  };
+  auto copy_v = [&](int st) {
+    uint16_t* to = vbuf[(st - first) & 1] + wave * 512;
+    copy_to_lds(vb[0] + st * kTreeStage, voff[0], to);
+    if (two) copy_to_lds(vb[1] + st * kTreeStage, voff[1], to + waves * 512);
+  };
+  copy_k(first);
   TreeTile t;
-  t.c = tree_query(a.q + ((size_t)node * a.heads + head) * kHeadDim + 8 * hb, t.qh, t.ql);
+  t.c = tree_query(query, t.qh, t.ql);
   const bool mine = tile * kTreeCols < rows;
   bool care = false;
   for (;; care = true) {
-    t.m = -INFINITY;
-    t.l = 0.f;
-#pragma unroll
-    for (int dt = 0; dt < 2; dt++)
-#pragma unroll
-      for (int i = 0; i < 16; i++) t.o[dt][i] = 0.f;
-    tree_landed();
+    tree_begin(t);
+    tree_landed<0>();
     __syncthreads();
-    if (first + 1 < end) tree_stage_k(copy, (first + 1) * kTreeStage, kbuf[1]);
-    tree_stage_v(copy, first * kTreeStage, vbuf[0]);
+    if (first + 1 < end) copy_k(first + 1);
+    copy_v(first);
     // What has been staged has landed when every wave has passed the barrier, and every wave is done with
     // the other buffers. Stage st lies in buffer (st - first) % 2.
-    auto turn = [&](int st, int now) {
-      tree_landed();
+    auto turn = [&](int st) {
+      tree_landed<0>();
       __syncthreads();
-      if (st + 2 < end) tree_stage_k(copy, (st + 2) * kTreeStage, kbuf[now]);
-      if (st + 1 < end) tree_stage_v(copy, (st + 1) * kTreeStage, vbuf[now ^ 1]);
+      if (st + 2 < end) copy_k(st + 2);
+      if (st + 1 < end) copy_v(st + 1);
     };
     f32x16 s[2], next[2];
     tree_scores(kbuf[0], t, col, hb, s);
     int st = first;
     for (; st + 2 <= clear; st += 2) {
-      turn(st, 0);
+      turn(st);
       tree_step(kbuf[1], vbuf[0], t, s, next, col, hb);
-      turn(st + 1, 1);
+      turn(st + 1);
       tree_step(kbuf[0], vbuf[1], t, next, s, col, hb);  // behind the last stage, of what the buffer holds, and not used
     }
     for (; st < end; st++) {
       const int now = (st - first) & 1;
-      turn(st, now);
+      turn(st);
       if (care) {
-        for (int i = threadIdx.x; i < kTreeStage * 8; i += waves * kWave) {
-          v4u* v = reinterpret_cast<v4u*>(vbuf[now]) + i;
-          tree_clip(*v, st * kTreeStage + 8 * ((i & 7) ^ (i >> 4 & 7)), total, a.past);
-        }
+        tree_clean<2>(vbuf[now], st * kTreeStage, total, a.past, threadIdx.x, waves * kWave);
         __syncthreads();
       }
-      tree_take(vbuf[now], t, s, col, hb, st * kTreeStage, a, mask);
+      const uint32_t win[2] = {tree_sees(a, mask, st * kTreeStage), tree_sees(a, mask, st * kTreeStage + 32)};
+      tree_take(vbuf[now], t, s, col, hb, st * kTreeStage, a, win);
       if (st + 1 < end) tree_scores(kbuf[now ^ 1], t, col, hb, s);
     }
     if (!__syncthreads_or(mine && tree_odd(t.o)) || care) break;
-    tree_stage_k(copy, first * kTreeStage, kbuf[0]);
+    copy_k(first);
   }
   if (!mine) return;
   tree_store(a, part, part_ml, out_buf[wave], kvh, tile * kTreeCols, split, splits, lane, t.m, pair_sum(t.l), t.o);
   if (care) {
-    tree_landed();  // the stores, which these overwrite
+    tree_landed<0>();  // the stores, which these overwrite
     tree_add_odd(a, part, kvh, tile * kTreeCols, 0, 1, first * kTreeStage, min(end * kTreeStage, total), split, splits);
   }
 }
@@ -699,12 +691,12 @@ struct TreePlan {
 TreePlan tree_plan(int nodes, int past, int heads, int kv_heads) {
   TreePlan t;
   const int cols = (nodes * (heads / kv_heads) + kTreeCols - 1) / kTreeCols, total = past + nodes;
-  const int steps = (total + kTreeKeys - 1) / kTreeKeys, stages = (total + kTreeStage - 1) / kTreeStage;
-  t.direct = cols < 4 || steps <= 64;
+  const int stages = (total + kTreeStage - 1) / kTreeStage;
+  t.direct = cols < 4 || stages <= 32;
   if (t.direct) {
     t.waves = 8;
     t.tiles = cols;
-    t.splits = steps <= 64 ? 1 : std::max(1, std::min(std::min(256 / (t.tiles * kv_heads), kMaxTreeSplits), (steps + 7) / 8));
+    t.splits = stages <= 32 ? 1 : std::max(1, std::min(std::min(256 / (t.tiles * kv_heads), kMaxTreeSplits), (stages + 7) / 8));
     return t;
   }
   t.tiles = (cols + kTreeWaves - 1) / kTreeWaves;

@@ -74,7 +74,8 @@ def test_attention_tree_refuses(hip, fake):
                                  ({"heads": 5}, E, "group evenly"), ({"kv_heads": 0}, E, "group evenly"),
                                  ({"heads": 1}, E, "group evenly"), ({"past": 16}, R, "exceeds capacity"),
                                  ({"past": 2**31 - 3}, R, "exceeds capacity"),
-                                 ({"nodes": 1 << 21, "past": 0, "capacity": 1 << 21}, E, "4194304 rows"), ({"q": fake.odd}, E, "aligned"),
+                                 ({"nodes": 1 << 21, "past": 0, "capacity": 1 << 21}, E, "4194304 rows"),
+                                 ({"capacity": (1 << 27) + 1}, E, "134217728 positions"), ({"q": fake.odd}, E, "aligned"),
                                  ({"kc": fake.byte}, E, "aligned"), ({"vc": fake.byte}, E, "aligned"), ({"out": fake.odd}, E, "aligned"),
                                  ({"mask": fake.odd}, E, "aligned"), ({"mask": hip.DeviceBuffer(fake, 0, 0)}, E, "the mask")]:
         _refused(hip, "attention_tree", ok, changes, error, what)
