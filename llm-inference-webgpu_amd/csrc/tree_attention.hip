@@ -681,7 +681,11 @@ __global__ __launch_bounds__(kBlock) void k_attn_tree_merge(TreeAttnArgs a, cons
 }
 
 namespace {
-// How a call is cut.
+// How a call is cut. Direct blocks read a range of keys once per tile of 32 rows, staged ones once per eight tiles;
+// in exchange those wait for each other at every stage. What decides is the work of a CU, tiles x 32-key steps.
+// Measured on 256 CUs, 14 heads of 2 kv heads, us direct / staged: 64 nodes at 4096 (14 a CU) 12.9 / 17.7, 128 at 8192
+// (56) 21.2 / 26.1, 256 at 4096 (56) 22.2 / 27.1, 64 at 32768 (112) 32.4 / 30.8, 256 at 8192 (112) 38.8 / 32.8, 128 at
+// 32768 (224) 54.8 / 42.9, 256 at 32768 (448) 102 / 72.
 struct TreePlan {
   bool direct;
   int waves;   // staged: column tiles of a block
@@ -691,19 +695,24 @@ struct TreePlan {
 TreePlan tree_plan(int nodes, int past, int heads, int kv_heads) {
   TreePlan t;
   const int cols = (nodes * (heads / kv_heads) + kTreeCols - 1) / kTreeCols, total = past + nodes;
-  const int stages = (total + kTreeStage - 1) / kTreeStage;
-  t.direct = cols < 4 || stages <= 32;
+  const int steps = (total + 31) / 32;
+  t.direct = (int64_t)cols * kv_heads * steps <= 256 * 100;
   if (t.direct) {
-    t.waves = 8;
+    t.waves = kTreeWaves;
     t.tiles = cols;
-    t.splits = stages <= 32 ? 1 : std::max(1, std::min(std::min(256 / (t.tiles * kv_heads), kMaxTreeSplits), (stages + 7) / 8));
+    // One range takes no merge, whose launch costs as much as two steps of each wave: 16 nodes at 256 7.4 us with
+    // one and 9.3 with two, at 1024 11.1 with one, 10.3 with four, 9.9 with eight.
+    const int room = 256 / std::min(256, t.tiles * kv_heads);
+    t.splits = steps <= 2 * kTreeWaves ? 1 : std::min(std::min(room, kMaxTreeSplits), std::max(8, (steps + 7) / 8));
     return t;
   }
+  const int stages = (total + kTreeStage - 1) / kTreeStage;
   t.tiles = (cols + kTreeWaves - 1) / kTreeWaves;
   t.waves = (cols + t.tiles - 1) / t.tiles;
   // A range costs its share of about 1 us a stage; each one more, 0.14 us per 1000 rows written and merged.
   const double want = sqrt(stages / (1.4e-4 * nodes * heads));
-  int s = std::max(1, std::min(std::min(256 / (t.tiles * kv_heads), kMaxTreeSplits), std::min(stages, (int)want)));
+  const int64_t blocks = (int64_t)t.tiles * kv_heads;
+  int s = (int)std::max<int64_t>(1, std::min(std::min<int64_t>(256 / blocks, kMaxTreeSplits), (int64_t)std::min<double>(stages, want)));
   for (int e = s; e > s * 3 / 4; e--)
     if (e * kv_heads % 8 == 0) {
       s = e;

@@ -59,7 +59,9 @@ def _check_attention(ctx, q, keys, values, see, past, heads, kv, mask=None, rms=
 
 SHAPES = [(1, 0, 14, 2), (1, 1, 14, 2), (1, 127, 2, 1), (2, 63, 4, 4), (5, 123, 14, 2), (7, 57, 1, 1), (9, 64, 9, 3),
           (16, 1024, 14, 2), (17, 31, 32, 2), (33, 0, 14, 2), (63, 500, 14, 2), (64, 1000, 4, 2), (65, 129, 14, 2), (100, 40, 7, 7),
-          (130, 2000, 14, 1), (200, 3, 4, 2), (3, 9000, 14, 2)]
+          (130, 2000, 14, 1), (200, 3, 4, 2), (3, 9000, 14, 2), (12, 500, 14, 2), (11, 513, 3, 3), (48, 3333, 14, 2),
+          # long enough and wide enough for the shared stages
+          (300, 6000, 20, 4), (700, 1900, 16, 1), (64, 32700, 14, 2), (65, 12863, 32, 1)]
 
 
 @pytest.mark.parametrize("nodes,past,heads,kv", SHAPES)
@@ -71,7 +73,8 @@ def test_attention_of_a_tree(ctx, nodes, past, heads, kv):
     _check_attention(ctx, q, keys, values, see, past, heads, kv)
 
 
-@pytest.mark.parametrize("nodes,past,heads,kv", [(1, 0, 2, 1), (5, 0, 14, 2), (40, 0, 14, 2), (70, 33, 4, 2), (129, 0, 2, 2)])
+@pytest.mark.parametrize("nodes,past,heads,kv", [(1, 0, 2, 1), (5, 0, 14, 2), (40, 0, 14, 2), (70, 33, 4, 2), (129, 0, 2, 2),
+                                                    (600, 0, 2, 2), (1300, 0, 32, 1)])
 def test_attention_of_any_mask(ctx, nodes, past, heads, kv):
     """Random bits, rows that see nothing, bits behind the last node."""
     rng = np.random.default_rng(nodes + past)
@@ -89,7 +92,8 @@ def test_attention_of_any_mask(ctx, nodes, past, heads, kv):
         assert not got[0].any()
 
 
-@pytest.mark.parametrize("nodes,past,heads,kv", [(6, 20, 14, 2), (40, 70, 4, 2), (96, 10, 14, 2)])
+@pytest.mark.parametrize("nodes,past,heads,kv", [(6, 20, 14, 2), (40, 70, 4, 2), (96, 10, 14, 2), (17, 3000, 14, 2),
+                                                    (64, 12900, 32, 1)])
 @pytest.mark.parametrize("what", [np.inf, -np.inf, np.nan])
 def test_attention_is_untouched_by_what_a_node_does_not_see(ctx, nodes, past, heads, kv, what):
     """Infinities and NaN in the K and V rows of hidden nodes change no bit; a node that sees an

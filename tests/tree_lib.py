@@ -33,20 +33,21 @@ def pack(see):
 
 
 def attention(q, keys, values, see, past, group):
-    """(out, sum of p |v|, largest sum of |q k| / 8 per row): q [n, heads, 64], keys [kv, P, 64], values [kv, 64, P]."""
+    """(out, sum of p |v|, largest sum of |q k| / 8 per row): q [n, heads, 64], keys [kv, P, 64], values [kv, 64, P].
+    A node that sees nothing gets zeros; what no node sees may be infinite or NaN."""
     n, heads, _ = q.shape
+    total = past + n
+    full = np.concatenate((np.ones((n, past), bool), see), 1)
     out, size, reach = np.zeros((n, heads, 64)), np.zeros((n, heads, 64)), np.zeros((n, heads, 1))
-    for i in range(n):
-        at = np.concatenate([np.arange(past), past + np.nonzero(see[i])[0]])
-        if not len(at):
-            continue
-        for h in range(heads):
-            k, v = keys[h // group][at].astype(np.float64), values[h // group][:, at].astype(np.float64)
-            s = k @ q[i, h].astype(np.float64) / 8
-            p = np.exp(s - s.max())
-            p /= p.sum()
-            out[i, h], size[i, h] = v @ p, np.abs(v) @ p
-            reach[i, h] = (np.abs(k) @ np.abs(q[i, h].astype(np.float64))).max() / 8
+    for h in range(heads):
+        k, v = (np.where(np.isfinite(t), t, 0).astype(np.float64) for t in (keys[h // group][:total], values[h // group][:, :total]))
+        qh = q[:, h].astype(np.float64)
+        s = np.where(full, qh @ k.T / 8, -np.inf)
+        m = s.max(1, keepdims=True)
+        p = np.where(full, np.exp(s - np.where(np.isfinite(m), m, 0)), 0)
+        p /= np.maximum(p.sum(1, keepdims=True), 1e-300)
+        out[:, h], size[:, h] = p @ v.T, p @ np.abs(v).T
+        reach[:, h, 0] = np.where(full, np.abs(qh) @ np.abs(k).T, 0).max(1) / 8
     return out, size, reach
 
 
