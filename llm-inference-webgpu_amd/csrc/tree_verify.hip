@@ -156,8 +156,10 @@ __device__ __forceinline__ uint32_t verify_hide(const VerifyArgs& a, int at, int
   return hide;
 }
 
-// grid (chunks, nodes). Bound: the f64 exponentials (20 f64 operations a logit, 8 cycles each) over the
-// logits' bytes: 64 rows of 151936 take 10.6 us without the exponentials, 13 us from cache alone.
+// grid (chunks, nodes). Bound: the f64 exponentials (20 f64 operations a logit, 8 cycles each) after the logits'
+// bytes: 64 rows of 151936 take 14 us, 10.6 without the exponentials, 13 from cache alone. (Tried: a table of 2^(j/64)
+// and a polynomial six operations shorter, 14.9; blocks that walk over two chunks with the next one's logits in
+// flight, 16.3; fewer blocks to a CU, 14.5-18.)
 template <bool GREEDY>
 __global__ __launch_bounds__(kRowsThreads) void k_verify_rows(VerifyArgs a, VerifyPart* __restrict__ part,
                                                               VerifyKid* __restrict__ kid) {
@@ -324,10 +326,21 @@ __global__ __launch_bounds__(kRowsThreads) void k_verify_residual(VerifyArgs a, 
   verify_load<kRowsThreads>(row, c0, a.vocab, verify_aligned(row), NAN, x);
   verify_load<kRowsThreads>(draft, c0, a.vocab, verify_aligned(draft), 0.f, q);
   const double k2 = 1.44269504088896340736 / a.temperature;
+  VerifyPart p[1];
+  VerifyKid child[kResiduals];
+  double u[kResiduals], sums[kResiduals];
+  verify_parts<1>(part + (size_t)node * chunks, 1, chunks, p);
+#pragma unroll
+  for (int r = 0; r < kResiduals; r++) {
+    if (r > round) break;
+    child[r] = kids_of[kid[r]];
+    u[r] = a.uniform[kid[r]];
+    sums[r] = 0.0;
+    if (r < round)
+      for (int c = lane; c < chunks; c += kWave) sums[r] += res[((size_t)r * a.nodes + node) * chunks + c];
+  }
   float max1[1];
   double sum1[1];
-  VerifyPart p[1];
-  verify_parts<1>(part + (size_t)node * chunks, 1, chunks, p);
   verify_row<1>(part + (size_t)node * chunks, p, 1, chunks, k2, max1, sum1);
   const float m = max1[0];
   const double inv_z = 1.0 / sum1[0];
@@ -335,10 +348,9 @@ __global__ __launch_bounds__(kRowsThreads) void k_verify_residual(VerifyArgs a, 
 #pragma unroll
   for (int r = 0; r < kResiduals; r++) {
     if (r > round) break;
-    const VerifyKid c = kids_of[kid[r]];
-    if (verify_accept(t, token_weight(c.logit, m, k2), inv_z, c.prob, a.uniform[kid[r]])) return;
+    if (verify_accept(t, token_weight(child[r].logit, m, k2), inv_z, child[r].prob, u[r])) return;
     t.a += t.f;
-    if (r < round) verify_reject(t, verify_residual_sum(res + ((size_t)r * a.nodes + node) * chunks, chunks));
+    if (r < round) verify_reject(t, team_sum<64>(sums[r]));
   }
   double s = 0.0;
   if (fabsf(m) < INFINITY) {
@@ -444,8 +456,35 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(VerifyArgs a, cons
   };
   if (tid == 0) a.path[0] = 0;
   if (point) {
-    // The first wave walks: a node's children to its lanes, tested all at once.
-    if (wave == 0) {
+    // The first wave walks: a node's children in its lanes, tested all at once. A token that an earlier child has weighs
+    // nothing, as it was rejected there; what is left at a child: the tokens that are none, and the children from it on.
+    if (wave == 0 && a.nodes <= kWave) {  // a node to a lane
+      const bool node = lane < a.nodes;
+      const int over = node ? parent[lane] : -1, x = node ? token[lane] : 0;
+      double w = over >= 0 ? weight[lane] : 0.0;
+      const double u = node ? uniform[lane] : 0.0;
+      for (;;) {
+        const uint64_t some = __ballot(over == at);
+        kids = some != 0;
+        if (!some) break;
+        for (uint64_t b = some; b; b &= b - 1) {
+          const int c = __builtin_ctzll(b);
+          if (over == at && lane > c && __builtin_amdgcn_readlane(x, c) == x) w = 0.0;
+        }
+        double left = row_sum[at], rest = 0.0;
+        for (uint64_t b = some; b;) {
+          const int c = 63 - __builtin_clzll(b);
+          b ^= (uint64_t)1 << c;
+          left += lane_value(w, c);
+          if (lane == c) rest = left;
+        }
+        const uint64_t good = __ballot(over == at && u * rest < w);
+        if (!good) break;
+        at = __builtin_ctzll(good);
+        if (lane == 0) a.path[count] = at;
+        count++;
+      }
+    } else if (wave == 0) {
       for (;;) {
         int n = 0;
         for (int j0 = at + 1; j0 < a.nodes; j0 += kWave) {
@@ -457,7 +496,6 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(VerifyArgs a, cons
         kids = n > 0;
         if (!n) break;
         wave_lds_handoff();
-        // A token that an earlier child has weighs nothing: it was rejected there.
         for (int b0 = 0; b0 < n; b0 += kWave) {
           const int i = b0 + lane < n ? list[b0 + lane] : 0, x = b0 + lane < n ? token[i] : -1;
           bool again = false;
@@ -466,7 +504,6 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(VerifyArgs a, cons
           if (again && x >= 0) weight[i] = 0.0;
         }
         wave_lds_handoff();
-        // What is left at a child: the tokens that are none, and the children from it on.
         double left = row_sum[at];
         int to = -1;
         for (int b0 = (n - 1) & ~(kWave - 1); b0 >= 0; b0 -= kWave) {
@@ -486,11 +523,11 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(VerifyArgs a, cons
         count++;
         wave_lds_handoff();
       }
-      if (lane == 0) {
-        walked[0] = at;
-        walked[1] = count;
-        walked[2] = kids;
-      }
+    }
+    if (tid == 0) {
+      walked[0] = at;
+      walked[1] = count;
+      walked[2] = kids;
     }
     __syncthreads();
     at = walked[0];
