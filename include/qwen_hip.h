@@ -225,7 +225,9 @@ int qh_argmax(qh_ctx* ctx, const float* d_v, int32_t n, int32_t* h_index);
  * output head qh_verify_tree walks the tree, and qh_kv_gather moves the accepted rows together, so
  * that the cache holds past + count positions and the walk's next token becomes the next node 0:
  *   qh_kv_gather(ctx, &kv, past, &kv, past, layers, kv_heads, head_dim, d_path, nodes, d_count)
- * All of them are asynchronous and can be captured into a graph from qh_stream. */
+ * All of them are asynchronous and can be captured into a graph from qh_stream. Scratch of attention
+ * and verification is the context's and grows at need (such a call waits for those before it); a
+ * capture gets scratch of its own, which is kept until qh_close. */
 
 /* Host-only: checks the parents (parent[0] = -1, 0 <= parent[i] < i; else QH_ERR_INVALID) and writes
  * each node's depth [nodes] and the mask of the nodes it sees, itself and its ancestors:
@@ -235,7 +237,8 @@ int qh_tree_plan(const int32_t* h_parent, int32_t nodes, int32_t* h_depth, uint6
 /* qh_rope of q and k at positions past + depth[i] and qh_kv_append of k and v at rows past + i, in
  * one launch. q [nodes, heads*head_dim], k, v [nodes, kv_heads*head_dim] f32; the rotated q goes to
  * d_q_out (which may be d_q), the rotated k only into the cache. Depths outside 0 .. nodes-1 are
- * taken as the nearest of those. past + nodes > capacity or > table_positions is QH_ERR_RANGE. */
+ * taken as the nearest of those. past + nodes > capacity or > table_positions is QH_ERR_RANGE;
+ * capacity at most 2^30, nodes * (heads + 2 kv_heads) * head_dim at most 2^31. */
 int qh_rope_append_tree(qh_ctx* ctx, const float* d_q, const float* d_k, const float* d_v, const float* d_cos,
                         const float* d_sin, int32_t table_positions, const int32_t* d_depth, float* d_q_out,
                         uint16_t* d_key_cache, uint16_t* d_value_cache, int32_t capacity, int32_t heads,
@@ -243,12 +246,13 @@ int qh_rope_append_tree(qh_ctx* ctx, const float* d_q, const float* d_k, const f
 
 /* Attention of the tree's queries over the caches of qh_kv_append: node i attends to positions
  * 0..past-1 and to position past + j for every bit j of its mask row (qh_tree_plan's layout; any
- * bits are allowed, those from `nodes` on are ignored). A node that sees nothing gets zeros. What a
- * node does not see has no influence on it, infinities and NaN included. q (rotated), out f32
- * [nodes, heads*64]; head h reads kv head h / (heads/kv_heads), any group; scale 1/8; head_dim must
- * be 64; buffers 16-byte aligned; nodes * heads at most 2^22, capacity
- * at most 2^27. q.k and p.v on f16 MFMA with q and p in
- * two f16 terms each, f32 sums (~1e-6 of the output). */
+ * bits are allowed, those from `nodes` on are ignored). A node that sees nothing, or only scores of
+ * -infinity, gets zeros. What a node does not see has no influence on it, infinities and NaN included;
+ * of what it sees, infinite values of nodes give the infinity or NaN of their sum and those of
+ * positions before past may give NaN. q (rotated), out f32 [nodes, heads*64]; head h reads kv head
+ * h / (heads/kv_heads), any group; scale 1/8; head_dim must be 64; buffers 16-byte aligned; nodes *
+ * heads at most 2^22, capacity at most 2^27. q.k and p.v on f16 MFMA with q and p in two f16 terms
+ * each, f32 sums (~1e-6 of the output). */
 int qh_attention_tree(qh_ctx* ctx, const float* d_q, const uint16_t* d_key_cache, const uint16_t* d_value_cache,
                       int32_t capacity, const uint64_t* d_mask, float* d_out, int32_t nodes, int32_t past,
                       int32_t heads, int32_t kv_heads, int32_t head_dim);
@@ -288,8 +292,8 @@ typedef struct {
  * thins or regrows one; within one (src and dst alike) it moves rows together: there an entry whose
  * source lies before its destination is left as it was, and the others read the rows as they were
  * before the call. Entries with a row outside the source are left as they were, as are all positions
- * that no entry names. head_dim a multiple of 8; caches 16-byte aligned with strides that are a
- * multiple of 8; two caches that overlap without being alike are QH_ERR_INVALID. */
+ * that no entry names. head_dim a multiple of 8 up to 1024; capacities at most 2^30; layers and
+ * kv_heads at most 65535; caches 16-byte aligned with strides that are a multiple of 8; two caches that overlap without being alike are QH_ERR_INVALID. */
 int qh_kv_gather(qh_ctx* ctx, const qh_kv* src, int32_t src_base, const qh_kv* dst, int32_t dst_base, int32_t layers,
                  int32_t kv_heads, int32_t head_dim, const int32_t* d_rows, int32_t n, const int32_t* d_count);
 

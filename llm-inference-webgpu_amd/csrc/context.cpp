@@ -171,6 +171,7 @@ int qh_close(qh_ctx* ctx) {
   hipStreamSynchronize(ctx->stream);
   hipFree(ctx->d_scratch);
   hipFree(ctx->d_tree);
+  for (const qh_ctx::TreePiece& p : ctx->tree_pieces) hipFree(p.ptr);
   hipHostFree(ctx->h_pinned);
   hipStreamDestroy(ctx->stream);
   delete ctx;
@@ -594,40 +595,52 @@ struct OnDevice {
 };
 
 // Scratch of one call: the context's, which its calls use in order and which grows to what they
-// ask for; or, while the stream is being captured, an allocation of the graph's own, so that
-// graphs may be replayed side by side and outlive the growth.
+// ask for. While the stream is being captured, a piece of that capture's own, kept until qh_close, so
+// that graphs may be replayed side by side, again before they have ended, and after the growth. (A
+// graph with memory nodes of its own cannot be launched again before its last launch has ended.)
 struct TreeScratch {
-  qh_ctx* ctx;
   void* ptr = nullptr;
-  bool own = false;
   hipError_t err = hipSuccess;
-  TreeScratch(qh_ctx* c, size_t bytes) : ctx(c) {
+  TreeScratch(qh_ctx* ctx, size_t bytes) {
     if (!bytes) return;
     hipStreamCaptureStatus capturing;
-    err = hipStreamIsCapturing(ctx->stream, &capturing);
+    unsigned long long id = 0;
+    err = hipStreamGetCaptureInfo(ctx->stream, &capturing, &id);
     if (err != hipSuccess) return;
     if (capturing != hipStreamCaptureStatusNone) {
-      err = hipMallocAsync(&ptr, bytes, ctx->stream);
-      own = err == hipSuccess;
+      for (const qh_ctx::TreePiece& p : ctx->tree_pieces)
+        if (p.capture == id && p.bytes >= bytes) ptr = p.ptr;
+      if (ptr) return;
+      hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;  // allocations are allowed
+      err = hipThreadExchangeStreamCaptureMode(&mode);
+      if (err != hipSuccess) return;
+      err = hipMalloc(&ptr, bytes);
+      const hipError_t back = hipThreadExchangeStreamCaptureMode(&mode);
+      if (err != hipSuccess) {
+        ptr = nullptr;
+        hipGetLastError();  // the next call's check is not to find it
+        return;
+      }
+      ctx->tree_pieces.push_back({id, ptr, bytes});
+      err = back;
       return;
     }
     if (bytes > ctx->tree_bytes) {
-      hipFree(ctx->d_tree);  // waits for the calls that use it
+      err = hipStreamSynchronize(ctx->stream);  // the calls that use it
+      if (err == hipSuccess) err = hipFree(ctx->d_tree);
+      if (err != hipSuccess) return;
       ctx->d_tree = nullptr;
       ctx->tree_bytes = 0;
       const size_t room = (bytes + bytes / 2 + ((size_t)4 << 20)) & ~(((size_t)1 << 20) - 1);
       err = hipMalloc(&ctx->d_tree, room);
       if (err != hipSuccess) {
         ctx->d_tree = nullptr;
-        hipGetLastError();  // the next call's check is not to find it
+        hipGetLastError();
         return;
       }
       ctx->tree_bytes = room;
     }
     ptr = ctx->d_tree;
-  }
-  ~TreeScratch() {
-    if (own) hipFreeAsync(ptr, ctx->stream);
   }
 };
 }  // namespace
@@ -645,6 +658,9 @@ int qh_rope_append_tree(qh_ctx* ctx, const float* d_q, const float* d_k, const f
            nodes, past, heads, kv_heads, head_dim);
   QH_CHECK((int64_t)heads + 2 * (int64_t)kv_heads <= (1 << 20) / head_dim, QH_ERR_INVALID,
            "rope_append_tree rows of %d + 2 x %d heads of %d are too wide", heads, kv_heads, head_dim);
+  QH_CHECK(capacity <= 1 << 30 && nodes <= (1 << 30) / ((heads + 2 * kv_heads) * (head_dim / 2)), QH_ERR_INVALID,
+           "rope_append_tree takes caches of up to 1073741824 positions (capacity %d) and 2^31 values (%d rows of %d)",
+           capacity, nodes, (heads + 2 * kv_heads) * head_dim);
   QH_CHECK((int64_t)past + nodes <= capacity, QH_ERR_RANGE, "cache holds %d of %d; cannot add %d", past, capacity,
            nodes);
   QH_CHECK((int64_t)past + nodes <= table_positions, QH_ERR_RANGE, "position %lld exceeds the %d-entry rope table",
@@ -728,6 +744,8 @@ int qh_kv_gather(qh_ctx* ctx, const qh_kv* src, int32_t src_base, const qh_kv* d
            layers, kv_heads, head_dim);
   QH_CHECK(n >= 0 && src_base >= 0 && dst_base >= 0 && src->capacity >= 1 && dst->capacity >= 1, QH_ERR_INVALID,
            "kv_gather needs n, both bases >= 0 and capacities >= 1");
+  QH_CHECK(src->capacity <= 1 << 30 && dst->capacity <= 1 << 30, QH_ERR_INVALID,
+           "kv_gather takes caches of up to 1073741824 positions (capacities %d and %d)", src->capacity, dst->capacity);
   const qh_kv* both[2] = {src, dst};
   size_t kel[2], vel[2];
   for (int i = 0; i < 2; i++) {

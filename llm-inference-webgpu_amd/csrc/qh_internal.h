@@ -7,6 +7,7 @@
 #include <cstddef>
 #include <cstdint>
 #include <string>
+#include <vector>
 
 #include "qwen_hip.h"
 
@@ -73,6 +74,12 @@ struct qh_ctx {
   // Scratch of the tree decoding operators, grown at need (TreeScratch).
   void* d_tree = nullptr;
   size_t tree_bytes = 0;
+  struct TreePiece {
+    unsigned long long capture;
+    void* ptr;
+    size_t bytes;
+  };
+  std::vector<TreePiece> tree_pieces;  // of captured calls
   // This device's copy of the no-allocation entry point's static scratch (or nullptr, and why).
   void* noalloc_scratch = nullptr;
   hipError_t noalloc_err = hipSuccess;

@@ -211,7 +211,7 @@ __device__ __noinline__ void tree_add_odd(TreeAttnArgs a, float* part, int kvh, 
     if (!any) continue;
     float* dst = splits > 1 ? part + tree_slot(kvh, rows, row, a.kv_heads, split) * kHeadDim
                             : a.out + ((size_t)node * a.heads + kvh * group + row % group) * kHeadDim;
-    dst[lane] = acc;
+    dst[lane] += acc;
   }
 }
 

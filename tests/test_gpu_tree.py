@@ -2,6 +2,7 @@
 (tree_lib.py), at the sizes, masks and values where it can go wrong, and a run of them together
 against a decode token by token."""
 import ctypes
+import threading
 
 import numpy as np
 import pytest
@@ -120,6 +121,29 @@ def test_attention_is_untouched_by_what_a_node_does_not_see(ctx, nodes, past, he
     touched = np.array([d % 2 == 0 or d == 1 for d in range(64)])
     assert (np.isnan(got[1][:, touched]).all() if np.isnan(what) else (got[1][:, touched] == what).all())
     assert np.isfinite(got[1][:, ~touched]).all()
+
+
+@pytest.mark.parametrize("nodes,past,heads,kv", [(6, 20, 14, 2), (20, 3000, 14, 2), (64, 12900, 32, 1)])
+def test_attention_adds_the_infinite_values_that_a_node_sees(ctx, nodes, past, heads, kv):
+    """Infinities of both signs in a dimension are NaN, of one sign that infinity, with a NaN before past NaN."""
+    rng = np.random.default_rng(nodes)
+    keys, values = _caches(rng, kv, past + nodes, past + nodes)
+    q = rng.standard_normal((nodes, heads * 64)).astype(np.float32)
+    _, see = T.plan(T.random_tree(rng, nodes))
+    see[-1] = False
+    see[-1, [1, 2, nodes - 1]] = True
+    see[:-1, [1, 2]] = False
+    want = _attend(ctx, q, keys, values, T.pack(see), past, heads, kv)
+    values[:, 3, past + 1] = np.inf
+    values[:, 4, past + 1], values[:, 4, past + 2] = np.inf, -np.inf
+    values[:, 5, past + 2] = -np.inf
+    values[:, 6, past + 1], values[:, 6, past // 2] = np.inf, np.nan
+    got = _attend(ctx, q, keys, values, T.pack(see), past, heads, kv)
+    assert (got[-1][:, 3] == np.inf).all() and (got[-1][:, 5] == -np.inf).all()
+    assert np.isnan(got[-1][:, 4]).all() and np.isnan(got[:, :, 6]).all()
+    same = np.ones(want.shape, bool)
+    same[-1, :, 3:6] = same[:, :, 6] = False
+    np.testing.assert_array_equal(got[same], want[same])
 
 
 @pytest.mark.parametrize("scale", [1e-6, 1e-3, 30.0, 1e4])
@@ -343,6 +367,21 @@ def test_verify_tree_with_nothing_left(ctx):
     assert _verify(ctx, logits, draft, tokens, parent, 1.0, u) == T.verify(logits, draft, tokens, parent, 1.0, u) == ([0], 7)
 
 
+@pytest.mark.parametrize("how", ["greedy", "lookup", "sampled"])
+@pytest.mark.parametrize("nodes,vocab", [(14, 9001), (64, 4100), (200, 9000)])
+def test_verify_tree_of_one_generation(ctx, how, nodes, vocab):
+    """All drafts under the root, some of them twice, with random numbers that reject most: more rejections than
+    have launches of their own, a draw from what they left."""
+    for seed in range(6):
+        rng = np.random.default_rng(seed)
+        logits, q, tokens, parent, u = _drafts(rng, nodes, vocab, how)
+        parent[1:] = 0
+        tokens[1:] = rng.choice(vocab, nodes - 1, p=(e := np.exp(logits[0].astype(np.float64))) / e.sum())
+        u[1:] = 1 - u[1:] * (0.02 if seed % 2 else 0.2)
+        t = 0.0 if how == "greedy" else 0.9
+        assert _verify(ctx, logits, q, tokens, parent, t, u) == T.verify(logits, q, tokens, parent, t, u), seed
+
+
 # ------------------------------------------------------------------- gather --
 
 def _kv(rng, layers, kv, hd, cap, pad=0):
@@ -412,6 +451,15 @@ def test_gather_between_caches(ctx, layers, kv, hd, src_cap, dst_cap, n):
     n = min(n, src_cap)
     for sb, db in ((0, 0), (src_cap - n, dst_cap - n)):  # a copy as it is
         _gather(ctx, src, src_cap, sb, dst, dst_cap, db, layers, kv, hd, None, n, None)
+
+
+def test_gather_of_wide_heads(ctx):
+    """The widest head, with rows over several steps of a block."""
+    rng = np.random.default_rng(1)
+    c = _kv(rng, 2, 2, 1024, 150, 8)
+    rows = np.sort(rng.choice(140, 90, replace=False)).astype(np.int32)
+    _gather(ctx, c, 150, 9, c, 150, 9, 2, 2, 1024, rows, 90, None)
+    _gather(ctx, c, 150, 0, _kv(rng, 2, 2, 1024, 91), 91, 1, 2, 2, 1024, rows, 90, 77)
 
 
 # -------------------------------------------------------------- all together --
@@ -590,3 +638,114 @@ def test_a_captured_step_replays(ctx, hip, nodes, past, how):
     ctx.done()
     rt.hipGraphExecDestroy(run)
     rt.hipGraphDestroy(graph)
+
+
+# ---------------------------------------------------------- calls side by side --
+
+def _attention_case(ctx, nodes, past, heads, kv, seed):
+    rng = np.random.default_rng(seed)
+    keys, values = _caches(rng, kv, past + nodes, past + nodes)
+    q = rng.standard_normal((nodes, heads * 64)).astype(np.float32)
+    _, see = T.plan(T.random_tree(rng, nodes))
+    bufs = [ctx.upload(np.ascontiguousarray(x)) for x in (q, keys, values, T.pack(see))] + [ctx.empty(q.nbytes)]
+
+    def call():
+        ctx.attention_tree(bufs[0], bufs[1], bufs[2], past + nodes, bufs[3], bufs[4], nodes, past, heads, kv)
+
+    return call, bufs[4]
+
+
+MIXED = [(5, 100, 14, 2), (64, 12900, 32, 1), (16, 1024, 14, 2), (300, 6000, 20, 4), (3, 9000, 14, 2), (130, 2000, 14, 1)]
+
+
+def test_scratch_that_grows_between_calls_in_flight(ctx, hip):
+    """A context's first calls, small and large, none waited for: the results of calls on their own."""
+    own = hip.GpuContext.create(0)
+    cases = [_attention_case(own, *shape, seed=i) for i, shape in enumerate(MIXED)]
+    own.done()
+    for call, _ in cases:
+        call()
+    first = [out.read() for _, out in cases]
+    for (call, out), want in zip(cases, first):
+        call()
+        np.testing.assert_array_equal(out.read(), want)
+    own.close()
+
+
+def test_two_contexts_on_two_threads(hip):
+    """Each thread's context has a stream and scratch of its own."""
+    contexts = [hip.GpuContext.create(0) for _ in range(2)]
+    cases = [[_attention_case(c, *shape, seed=10 * k + i) for i, shape in enumerate(MIXED)] for k, c in enumerate(contexts)]
+    want = []
+    for mine in cases:
+        want.append([])
+        for call, out in mine:
+            call()
+            want[-1].append(out.read())
+    errors = []
+
+    def run(k):
+        try:
+            for _ in range(5):
+                order = np.random.default_rng(k).permutation(len(MIXED))
+                for i in order:
+                    cases[k][i][0]()
+                for i in order:
+                    np.testing.assert_array_equal(cases[k][i][1].read(), want[k][i])
+        except BaseException as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors[0]
+    for c in contexts:
+        c.close()
+
+
+@pytest.mark.parametrize("captured_by", [(0, 1), (0, 0)])
+def test_two_graphs_side_by_side(hip, captured_by):
+    """Two graphs whose calls need scratch, captured by two contexts or by one, replayed at once on two streams, again
+    before they have ended, with direct calls between."""
+    rt = _runtime()
+    contexts = [hip.GpuContext.create(0) for _ in range(2)]
+    cases = [[_attention_case(contexts[c], *shape, seed=20 * k + i) for i, shape in enumerate(MIXED)] for k, c in enumerate(captured_by)]
+    want, graphs, runs = [], [], []
+    for c, mine in zip((contexts[c] for c in captured_by), cases):
+        want.append([])
+        for call, out in mine:
+            call()
+            want[-1].append(out.read())
+        graph, run = ctypes.c_void_p(), ctypes.c_void_p()
+        c.done()
+        assert rt.hipStreamBeginCapture(c.stream, 1) == 0  # thread local
+        for call, _ in mine:
+            call()
+        assert rt.hipStreamEndCapture(c.stream, ctypes.byref(graph)) == 0
+        assert rt.hipGraphInstantiate(ctypes.byref(run), graph, None, None, 0) == 0
+        graphs.append(graph)
+        runs.append(run)
+    for turn in range(4):
+        for mine in cases:
+            for _, out in mine:
+                nan = np.full(out.nbytes // 4, np.nan, np.float32)
+                assert out.ctx.lib.qh_upload(out.ctx.handle, out.ptr, nan.ctypes.data, nan.nbytes) == 0
+        for _ in range(3):
+            for c, run in zip(contexts, runs):
+                assert rt.hipGraphLaunch(run, c.stream) == 0
+        for c in contexts:
+            c.done()
+        for k, mine in enumerate(cases):
+            for (call, out), w in zip(mine, want[k]):
+                np.testing.assert_array_equal(out.read(), w)
+            if turn % 2:
+                mine[turn][0]()
+    for c in contexts:
+        c.done()
+    for graph, run in zip(graphs, runs):
+        rt.hipGraphExecDestroy(run)
+        rt.hipGraphDestroy(graph)
+    for c in contexts:
+        c.close()

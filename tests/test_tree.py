@@ -61,6 +61,8 @@ def test_rope_append_tree_refuses(hip, fake):
                                  ({"kv_heads": 0}, E, "kv_heads=0"), ({"head_dim": 7}, E, "head_dim=7"),
                                  ({"heads": 1 << 20}, E, "too wide"), ({"past": 16}, R, "cannot add 5"),
                                  ({"past": 2**31 - 1}, R, "cannot add"), ({"table_positions": 14}, R, "rope table"),
+                                 ({"capacity": (1 << 30) + 1}, E, "1073741824 positions"),
+                                 ({"capacity": 1 << 30, "table_positions": 1 << 30, "past": 0, "nodes": (1 << 22) + 1}, E, "2\\^31 values"),
                                  ({"q": hip.DeviceBuffer(fake, 0, 0)}, E, "needs q"),
                                  ({"vc": hip.DeviceBuffer(fake, 0, 0)}, E, "both caches")]:
         _refused(hip, "rope_append_tree", ok, changes, error, what)
@@ -110,6 +112,7 @@ def test_kv_gather_refuses(hip, fake):
             ({"dst_base": -1}, E, "bases"), ({"dst_base": 13}, R, "cannot write 4 at 13"),
             ({"dst_base": 2**31 - 1}, R, "cannot write"), ({"src_base": 13, "rows": None}, R, "cannot read 4 at 13"),
             ({"src_base": 17}, R, "cannot read"), ({"src": kv(8)}, E, "aligned"), ({"dst": kv(far, far + 4)}, E, "aligned"),
+            ({"src": kv(capacity=2**30 + 1)}, E, "1073741824"), ({"dst": kv(far, far + (1 << 20), 2**31 - 1)}, E, "1073741824"),
             ({"src": kv(capacity=0)}, E, "capacities"), ({"layers": 2}, E, "strides"),
             ({"layers": 2, "src": kv(ks=2052, vs=8192), "dst": kv(far, far + (1 << 20), 16, 2048, 8192)}, E, "strides"),
             ({"src": kv(ks=2**20, vs=2**20), "dst": kv(far, far + (1 << 20), 16, 2040, 8192), "layers": 2}, E, "strides"),
