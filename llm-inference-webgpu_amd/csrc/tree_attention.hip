@@ -13,10 +13,9 @@
 // first scaled by a power of two to below 2^14, so no finite q leaves f16's range and small ones keep
 // their bits; p is scaled by 2^13, so a weight of 2^-27 of the row's largest is still a normal f16 number.
 //
-// Block: WQ x WK waves, WQ column tiles by WK runs of keys; wave (t, k) takes the 32-key steps k, k + WK, ...
-// of the block's range for column tile t, with an online softmax, and the WK states of a tile merge
-// through LDS in order. Ranges of a long context go to blocks of their own (grid x), whose states a
-// second launch merges in order.
+// Two kernels (tree_plan chooses): direct ones, whose waves deal the keys of one tile among them, and staged ones,
+// whose waves have a tile each and share the keys. Ranges of a long context go to blocks of their own, whose
+// states (o, m, l) k_attn_tree_merge joins in order; no sum depends on which block is first.
 #include <algorithm>
 #include <cmath>
 
@@ -366,8 +365,11 @@ __device__ __forceinline__ void tree_take(const uint16_t* vbuf, TreeTile& t, f32
 }
 
 // Short contexts and few rows: a block of WK waves has a tile of rows and a range of keys, and wave w takes the
-// 32-key stages w, w + WK, ... of it in two buffers of its own, the next one on its way. The waves' states merge through LDS, each wave merging its share of the dimensions over
-// all of them in order.
+// 32-key stages w, w + WK, ... of it in two buffers of its own, the next one on its way, with no barrier. The waves'
+// states merge through LDS, each wave merging its share of the dimensions over all of them in order.
+// Bound: latency (a launch, q and a stage from memory, the joining of the waves). 14 heads of 2 kv heads: 5 nodes at
+// 123 (4 stages, one launch) 6.0 us; 16 at 1024 7.6 and 63 at 4097 10.3, and 3.7 and 3.9 for the merge. (Operands
+// straight from the caches instead of through LDS: 12.7 for 11.1 at 16 nodes, with the merge.)
 template <int WK>
 __global__ __launch_bounds__(kWave * WK, 2) void k_attn_tree_direct(TreeAttnArgs a, float* __restrict__ part,
                                                                   float* __restrict__ part_ml) {
@@ -502,7 +504,12 @@ __global__ __launch_bounds__(kWave * WK, 2) void k_attn_tree_direct(TreeAttnArgs
 
 // Long contexts and many rows: a block's waves, a column tile each, share the stages. A stage's scores are made while
 // the weights of the one before it are: its K is copied one turn ahead of its V, and the products' matrix
-// instructions have the exponentials to run under.
+// instructions have the exponentials to run under. A barrier a stage: eight waves read what one copied, 64 KB a
+// CU's turn instead of 512.
+// Bound: the matrix cores, at the clock that they leave: 32 instructions of 32 cycles a wave and stage, with the two
+// terms of q and p, are 44 us of 256 nodes at 32512 (60 GF; 14 heads of 2 kv heads) at the rate of a large product;
+// the kernel takes 68, 1.85 us a stage of two waves a SIMD. 64 nodes at 32700: 28.2, of which a block's stages 16, q
+// 2.5, the partials 1. (With one term of q 61, of p 58, of both 51, for weights and scores that are off by 2^-12.)
 constexpr int kTreeStage = 64;
 constexpr int kTreeWaves = 8;
 
@@ -657,7 +664,9 @@ __global__ __launch_bounds__(kWave * kTreeWaves, 2) void k_attn_tree_staged(Tree
 }
 
 // The merge of a row's `splits` partials, a wave a row: lane (k, d) of 4 x 16 sums dimensions 4 d .. +3 over splits
-// k, k + 4, ..., and the four sums are added in order.
+// k, k + 4, ..., and the four sums are added in order: o = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s.
+// Bound: latency of two loads behind a launch (224 rows of 8 ranges 3.7 us, 882 of 9 3.9); 5.4 for 896 rows of 60, 14 MB.
+// Joined by the last block of a tile instead, the states would cross the XCDs through fences that take as long.
 __global__ __launch_bounds__(kBlock) void k_attn_tree_merge(TreeAttnArgs a, const float* __restrict__ part,
                                                             const float* __restrict__ part_ml, int splits) {
   const int lane = threadIdx.x & (kWave - 1), group = a.heads / a.kv_heads, rows = a.nodes * group;
