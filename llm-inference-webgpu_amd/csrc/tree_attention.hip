@@ -668,8 +668,11 @@ __global__ __launch_bounds__(kWave * kTreeWaves, 2) void k_attn_tree_staged(Tree
 
 // The merge of a row's `splits` partials, a wave a row: lane (k, d) of 4 x 16 sums dimensions 4 d .. +3 over splits
 // k, k + 4, ..., and the four sums are added in order: o = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s.
-// Bound: latency of two loads behind a launch (224 rows of 8 ranges 3.7 us, 882 of 9 3.9); 5.4 for 896 rows of 60, 14 MB.
+// kFlight of a lane's splits are loaded at once, the first ones before the maximum is known: 1 up to 4 splits, 4 up to 16, 8
+// beyond (64 of 14 rows: 12.2 us with 8 and 15.2 with 4, the attention included; 2 of 3584: 24.9 and 24.0).
+// Bound: latency of a load behind a launch; bytes for many rows (14 MB for 896 rows of 60 ranges).
 // Joined by the last block of a tile instead, the states would cross the XCDs through fences that take as long.
+template <int kFlight>
 __global__ __launch_bounds__(kBlock) void k_attn_tree_merge(TreeAttnArgs a, const float* __restrict__ part,
                                                             const float* __restrict__ part_ml, int splits) {
   const int lane = threadIdx.x & (kWave - 1), group = a.heads / a.kv_heads, rows = a.nodes * group;
@@ -679,19 +682,38 @@ __global__ __launch_bounds__(kBlock) void k_attn_tree_merge(TreeAttnArgs a, cons
   const size_t step = (size_t)a.kv_heads * rows;  // from split to split
   const float* p = part + (size_t)at * kHeadDim + 4 * d;
   const f32x2* ml = reinterpret_cast<const f32x2*>(part_ml) + at;
+  f32x2 w2[kFlight];
+  v4f x[kFlight];
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int j = 0; j < kFlight; j++) {
+      const int s = s0 + 4 * j, in = min(s, splits - 1);
+      w2[j] = ml[in * step];
+      x[j] = *reinterpret_cast<const v4f*>(p + in * step * kHeadDim);
+      if (s < splits) continue;
+      w2[j] = f32x2{-INFINITY, 0.f};
+      x[j] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+  };
+  load(k);
   float mx = -INFINITY;
-  for (int s = lane; s < splits; s += kWave) mx = fmaxf(mx, ml[s * step].x);
+#pragma unroll
+  for (int j = 0; j < kFlight; j++) mx = fmaxf(mx, w2[j].x);
+  for (int s = 4 * kFlight + lane; s < splits; s += kWave) mx = fmaxf(mx, ml[s * step].x);
   mx = team_max<64>(mx);
   float l = 0.f;
   v4f o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int s = k; s < splits; s += 4) {
-    const f32x2 w2 = ml[s * step];
-    const v4f x = *reinterpret_cast<const v4f*>(p + s * step * kHeadDim);
-    const float w = w2.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w2.x - mx);
-    l = fmaf(w, w2.y, l);
+  for (int s0 = k;;) {
 #pragma unroll
-    for (int r = 0; r < 4; r++) o[r] = fmaf(w, x[r], o[r]);
+    for (int j = 0; j < kFlight; j++) {
+      const float w = w2[j].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w2[j].x - mx);
+      l = fmaf(w, w2[j].y, l);
+#pragma unroll
+      for (int r = 0; r < 4; r++) o[r] = fmaf(w, x[j][r], o[r]);
+    }
+    s0 += 4 * kFlight;
+    if (s0 - k >= splits) break;
+    load(s0);
   }
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
@@ -724,10 +746,13 @@ TreePlan tree_plan(int nodes, int past, int heads, int kv_heads) {
   if (t.direct) {
     t.waves = kTreeWaves;
     t.tiles = cols;
-    // One range takes no merge, whose launch costs as much as two steps of each wave: 16 nodes at 256 7.4 us with
-    // one and 9.3 with two, at 1024 11.1 with one, 10.3 with four, 9.9 with eight.
+    // In us: a step takes its block 0.15, a merge 2.4, 0.045 a range and 0.5 per 1000 rows. So sqrt(3.3 steps) ranges, as
+    // the CUs allow, or one without a merge. Measured with 1 / 4 / 8 / 16 / 32 / 64: 5 nodes at 512 8.4 / 9.0 / 9.1 / 9.4,
+    // at 1040 10.9 / 10.1 / 10.0 / 9.2 / 9.6, at 4097 25.5 / 13.8 / 11.3 / 10.4 / 10.3 / 11.0, one at 32768 8 to 128: 27.3 /
+    // 18.2 / 13.3 / 12.2 / 14.1; 200 nodes at 1024, 16 heads of one kv head, with 1 / 2: 11.7 / 13.3.
     const int room = 256 / std::min(256, t.tiles * kv_heads);
-    t.splits = steps <= 2 * kTreeWaves ? 1 : std::min(std::min(room, kMaxTreeSplits), std::max(8, (steps + 7) / 8));
+    t.splits = std::min(std::min(room, kMaxTreeSplits), (int)(sqrt(3.3 * steps) + 0.5));
+    if (0.15 * steps <= 0.15 * steps / t.splits + 2.4 + 0.045 * t.splits + 0.0005 * nodes * heads) t.splits = 1;
     return t;
   }
   const int stages = (total + kTreeStage - 1) / kTreeStage;
@@ -763,7 +788,10 @@ hipError_t launch_attention_tree(hipStream_t s, const TreeAttnArgs& a, float* pa
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || t.splits == 1) return e;
   const int rows = a.nodes * a.heads;
-  hipLaunchKernelGGL(k_attn_tree_merge, dim3((rows + 3) / 4), dim3(kBlock), 0, s, a, part, ml, t.splits);
+  const dim3 grid((rows + 3) / 4), block(kBlock);
+  if (t.splits <= 4) hipLaunchKernelGGL((k_attn_tree_merge<1>), grid, block, 0, s, a, part, ml, t.splits);
+  else if (t.splits <= 16) hipLaunchKernelGGL((k_attn_tree_merge<4>), grid, block, 0, s, a, part, ml, t.splits);
+  else hipLaunchKernelGGL((k_attn_tree_merge<8>), grid, block, 0, s, a, part, ml, t.splits);
   return hipGetLastError();
 }
 
