@@ -368,8 +368,8 @@ __device__ __forceinline__ void tree_take(const uint16_t* vbuf, TreeTile& t, f32
 // 32-key stages w, w + WK, ... of it in two buffers of its own, the next one on its way, with no barrier. The waves'
 // states merge through LDS, each wave merging its share of the dimensions over all of them in order.
 // Bound: latency (a launch, q and a stage from memory, the joining of the waves). 14 heads of 2 kv heads: 5 nodes at
-// 123 (4 stages, one launch) 6.0 us; 16 at 1024 7.6 and 63 at 4097 10.3, and 3.7 and 3.9 for the merge. (Operands
-// straight from the caches instead of through LDS: 12.7 for 11.1 at 16 nodes, with the merge.)
+// 123 (4 stages, one launch) 6.0 us; 16 at 1024 6.9 and 63 at 4097 10.3, and 3.3 and 3.6 for the merge. (Operands
+// straight from the caches instead of through LDS: 12.7 for 11.1 at 16 nodes, both launches of an earlier form.)
 template <int WK>
 __global__ __launch_bounds__(kWave * WK, 2) void k_attn_tree_direct(TreeAttnArgs a, float* __restrict__ part,
                                                                   float* __restrict__ part_ml) {
