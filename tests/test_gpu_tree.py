@@ -382,6 +382,20 @@ def test_verify_tree_of_one_generation(ctx, how, nodes, vocab):
         assert _verify(ctx, logits, q, tokens, parent, t, u) == T.verify(logits, q, tokens, parent, t, u), seed
 
 
+@pytest.mark.parametrize("how", ["greedy", "lookup", "sampled"])
+def test_verify_tree_of_the_largest_vocabulary(ctx, how):
+    vocab = 1 << 24
+    rng = np.random.default_rng(11)
+    logits = rng.standard_normal((3, vocab), np.float32) * np.float32(2.5)
+    draft = None
+    if how == "sampled":
+        draft = np.exp(logits[:, ::-1]) / np.float32(4e8)  # of other tokens than the target's
+    parent, tokens = np.array([-1, 0, 0], np.int32), np.array([0, int(logits[0].argmin()), vocab - 1], np.int32)
+    for u in (np.array([0.3, 0.99, 0.9]), np.array([0.97, 0.99, 0.0]), np.array([1 - 2.0**-53, 0.99, 0.99])):
+        t = 0.0 if how == "greedy" else 0.7
+        assert _verify(ctx, logits, draft, tokens, parent, t, u) == T.verify(logits, draft, tokens, parent, t, u)
+
+
 # ------------------------------------------------------------------- gather --
 
 def _kv(rng, layers, kv, hd, cap, pad=0):
@@ -460,6 +474,50 @@ def test_gather_of_wide_heads(ctx):
     rows = np.sort(rng.choice(140, 90, replace=False)).astype(np.int32)
     _gather(ctx, c, 150, 9, c, 150, 9, 2, 2, 1024, rows, 90, None)
     _gather(ctx, c, 150, 0, _kv(rng, 2, 2, 1024, 91), 91, 1, 2, 2, 1024, rows, 90, 77)
+
+
+def test_append_and_gather_behind_four_billion_bytes(ctx):
+    """The last kv head's rows start behind 2^32 bytes and 2^31 values, the tables' rows behind 2^30 bytes."""
+    rng = np.random.default_rng(7)
+    nodes, heads, kv, cap = 6, 8, 4, 12_000_000
+    past = cap - 70
+    keys, values, cos, sin = (ctx.empty(b) for b in (kv * cap * 128, kv * 64 * _vstride(cap) * 2, cap * 128, cap * 128))
+    q, k, v = (rng.standard_normal((nodes, h * 64)).astype(np.float32) for h in (heads, kv, kv))
+    depth = np.array([0, 1, 1, 2, 3, 2], np.int32)
+    angle = rng.standard_normal((nodes, 32))
+
+    def piece(call, buf, offset, a):
+        assert call(ctx.handle, *((a.ctypes.data, buf.ptr + offset) if call is ctx.lib.qh_download else
+                                  (buf.ptr + offset, a.ctypes.data)), a.nbytes) == 0
+        return a
+
+    for t, f in ((cos, np.cos), (sin, np.sin)):
+        piece(ctx.lib.qh_upload, t, past * 128, f(angle).astype(np.float32))
+    bufs = [ctx.upload(x) for x in (q, k, v, depth, np.array([0, 1, 3, 5], np.int32))]
+    out = ctx.empty(q.nbytes)
+    ctx.rope_append_tree(*bufs[:3], cos, sin, cap, bufs[3], out, keys, values, cap, heads, kv, 64, past, nodes)
+
+    def rows(n):
+        return (np.stack([piece(ctx.lib.qh_download, keys, (h * cap + past) * 128, np.empty((n, 64), np.float16)) for h in range(kv)]),
+                np.stack([[piece(ctx.lib.qh_download, values, ((h * 64 + d) * _vstride(cap) + past) * 2, np.empty(n, np.float16))
+                           for d in range(64)] for h in range(kv)]))
+
+    got_k, got_v = rows(nodes)
+    np.testing.assert_array_equal(got_v, v.reshape(nodes, kv, 64).transpose(1, 2, 0).astype(np.float16))
+    x = k.reshape(nodes, kv, 2, 32).astype(np.float64)
+    turn = np.exp(1j * angle)[depth][:, None]
+    want = (x[:, :, 0] + 1j * x[:, :, 1]) * turn
+    want = np.concatenate((want.real, want.imag), 2).transpose(1, 0, 2)
+    # the tables' and the products' roundings to f32 of values below 8, then half an f16 step
+    assert (np.abs(got_k - want) <= 6 * 2.0**-24 * 8 + np.abs(want) * 2.0**-11 + 2.0**-25).all()
+    c = ctx.kv_list(keys, values, cap)
+    ctx.kv_gather(c, past, c, past, 1, kv, 64, bufs[4], 4, None)
+    new_k, new_v = rows(nodes)
+    take = [0, 1, 3, 5, 4, 5]  # what lies behind the four stays
+    np.testing.assert_array_equal(new_k, got_k[:, take])
+    np.testing.assert_array_equal(new_v, got_v[..., take])
+    for b in (keys, values, cos, sin):
+        b.free()
 
 
 # -------------------------------------------------------------- all together --
@@ -705,8 +763,8 @@ def test_two_contexts_on_two_threads(hip):
         c.close()
 
 
-@pytest.mark.parametrize("captured_by", [(0, 1), (0, 0)])
-def test_two_graphs_side_by_side(hip, captured_by):
+@pytest.mark.parametrize("captured_by,mode", [((0, 1), 1), ((0, 0), 1), ((0, 1), 0)])
+def test_two_graphs_side_by_side(hip, captured_by, mode):
     """Two graphs whose calls need scratch, captured by two contexts or by one, replayed at once on two streams, again
     before they have ended, with direct calls between."""
     rt = _runtime()
@@ -720,7 +778,7 @@ def test_two_graphs_side_by_side(hip, captured_by):
             want[-1].append(out.read())
         graph, run = ctypes.c_void_p(), ctypes.c_void_p()
         c.done()
-        assert rt.hipStreamBeginCapture(c.stream, 1) == 0  # thread local
+        assert rt.hipStreamBeginCapture(c.stream, mode) == 0  # thread local or global
         for call, _ in mine:
             call()
         assert rt.hipStreamEndCapture(c.stream, ctypes.byref(graph)) == 0
