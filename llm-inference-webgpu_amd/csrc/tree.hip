@@ -55,17 +55,20 @@ hipError_t launch_rope_append_tree(hipStream_t s, const RopeTreeArgs& a) {
 
 // ------------------------------------------------------------------- gather --
 // dst[dst_base + j] = src[src_base + rows[j]]. A block takes a step of key rows (16-byte pieces, kKeyPieces a thread)
-// or of value positions: a thread eight of a dimension's row, which are 2-byte loads from a run of the source that its
-// neighbours share and one 16-byte store, for several dimensions: kDimsBetween a block between two caches, kDimsInPlace
-// in place.
+// or of value positions: a thread eight of a dimension's row, in runs of kRun, whose 2-byte loads fall into lines that its
+// neighbours share and which it stores at once, for kValueDims dimensions.
 // Between caches the bound is HBM: 16384 of 32768 positions, every second on average, of 24 layers of 2 kv heads take
-// 102 us. Read and written are 402 MB, 79 us of a copy; but whole lines of values are read where half of their
-// positions are kept, 503 MB, 99 us. Dimensions a block: 8 135 us, 4 102, 2 115; without nontemporal stores 144 for 135.
+// 93 us. Read and written are 402 MB, 79 us of a copy; but whole lines of values are read where half of their
+// positions are kept, 503 MB, 99 us of one. Runs of 8 / 4 / 2 with four dimensions: 101 / 95 / 93, 4000 of 32768 81 / 75 /
+// 68, 1000 of 2048 10.1 / 7.6 / 7.2: the fewer source lines an instruction touches, the better. Four dimensions or two,
+// in runs of 2: 250 of 512 4.9 / 5.4, 1000 of 2048 7.2 / 7.9, 4000 of 8192 24.2 / 23.1, 4000 of 32768 68 / 62, hence
+// kManyRows; eight 98 for 93. Ordinary stores for nontemporal ones 29.0 for 24.2 at 4000 of 8192.
 // In place the blocks of a (layer, head, part) are one, which walks its steps upward, a step's reads all before its
 // writes: an entry's source is never before its destination (others are left), so no step reads what an earlier one
-// wrote. Bound: the latency of a launch, a count, a row and a copy after each other: 6 of 64 nodes 4.3 us (0.1 MB).
+// wrote. Bound: the latency of a launch, a count, a row and a copy after each other: 6 of 64 nodes 4.3 us (0.1 MB). Runs
+// of 8, 4 and 2 are alike there (1000 of 2048 19.7, 19.3, 19.1).
 constexpr int kKeyPieces = 4;
-constexpr int kDimsBetween = 4, kDimsInPlace = 8;
+constexpr int kDimsInPlace = 8, kManyRows = 2048;
 
 struct GatherCut {
   int key_blocks, value_blocks;  // along grid x (value_blocks per group of dimensions)
@@ -79,8 +82,9 @@ __device__ __forceinline__ int gather_source(const GatherArgs& a, int n, int j) 
   return a.in_place && a.src_base + r < a.dst_base + j ? -1 : a.src_base + r;
 }
 
-template <bool IN_PLACE, int kValueDims>
+template <bool IN_PLACE, int kValueDims, int kRun>
 __global__ __launch_bounds__(kBlock) void k_kv_gather(GatherArgs a, GatherCut cut) {
+  constexpr int kRuns = 8 / kRun;
   const int h = blockIdx.y, tid = threadIdx.x;
   const size_t layer = blockIdx.z;
   const int n = a.count ? min(max(*a.count, 0), a.n) : a.n;
@@ -114,36 +118,48 @@ __global__ __launch_bounds__(kBlock) void k_kv_gather(GatherArgs a, GatherCut cu
   uint16_t* dst = a.dst_value + layer * a.dst_value_stride + row0 * dst_stride;
   const int first = a.dst_base / 8, octets = (a.dst_base + n + 7) / 8 - first;
   for (int o0 = block % cut.value_blocks * cut.octets; o0 < octets; o0 += cut.octets) {
-    const int d0 = 8 * (first + o0 + at);  // destination positions d0 .. d0+7
-    int p[8], some = -1, all = 0;
+    int d0[kRuns], p[kRuns][kRun], some[kRuns], all[kRuns];  // destination positions d0 .. d0 + kRun - 1
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      p[e] = gather_source(a, n, d0 + e - a.dst_base);
-      some = max(some, p[e]);
-      all |= p[e];
+    for (int r = 0; r < kRuns; r++) {
+      d0[r] = 8 * (first + o0) + kRun * (r * cut.octets + at);
+      some[r] = -1;
+      all[r] = 0;
+#pragma unroll
+      for (int e = 0; e < kRun; e++) {
+        p[r][e] = gather_source(a, n, d0[r] + e - a.dst_base);
+        some[r] = max(some[r], p[r][e]);
+        all[r] |= p[r][e];
+      }
     }
-    uint16_t x[kValueDims][8];
+    uint16_t x[kValueDims][kRuns][kRun];
 #pragma unroll
     for (int k = 0; k < kValueDims; k++) {
       const int d = tid / cut.octets + k * turn;
-      if (d < dims && some >= 0) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[k][e] = src[(size_t)d * src_stride + max(p[e], 0)];
-      }
+      for (int r = 0; r < kRuns; r++)
+        if (d < dims && some[r] >= 0) {
+#pragma unroll
+          for (int e = 0; e < kRun; e++) x[k][r][e] = src[(size_t)d * src_stride + max(p[r][e], 0)];
+        }
     }
     if (IN_PLACE) __syncthreads();
 #pragma unroll
     for (int k = 0; k < kValueDims; k++) {
       const int d = tid / cut.octets + k * turn;
-      if (d >= dims || some < 0) continue;
-      uint16_t* y = dst + (size_t)d * dst_stride + d0;
-      if (all >= 0) {
-        __builtin_nontemporal_store(v4u{x[k][0] | (uint32_t)x[k][1] << 16, x[k][2] | (uint32_t)x[k][3] << 16,
-                                         x[k][4] | (uint32_t)x[k][5] << 16, x[k][6] | (uint32_t)x[k][7] << 16}, reinterpret_cast<v4u*>(y));
-      } else {
 #pragma unroll
-        for (int e = 0; e < 8; e++)
-          if (p[e] >= 0) y[e] = x[k][e];
+      for (int r = 0; r < kRuns; r++) {
+        if (d >= dims || some[r] < 0) continue;
+        uint16_t* y = dst + (size_t)d * dst_stride + d0[r];
+        if (all[r] >= 0) {
+          uint32_t w __attribute__((ext_vector_type(kRun / 2)));
+#pragma unroll
+          for (int e = 0; e < kRun; e += 2) w[e / 2] = x[k][r][e] | (uint32_t)x[k][r][e + 1] << 16;
+          __builtin_nontemporal_store(w, reinterpret_cast<decltype(w)*>(y));
+        } else {
+#pragma unroll
+          for (int e = 0; e < kRun; e++)
+            if (p[r][e] >= 0) y[e] = x[k][r][e];
+        }
       }
     }
     if (!IN_PLACE) return;
@@ -152,16 +168,17 @@ __global__ __launch_bounds__(kBlock) void k_kv_gather(GatherArgs a, GatherCut cu
 
 hipError_t launch_kv_gather(hipStream_t s, const GatherArgs& a) {
   GatherCut cut;
-  const int kValueDims = a.in_place ? kDimsInPlace : kDimsBetween;
+  const int kValueDims = a.in_place ? kDimsInPlace : a.n < kManyRows ? 4 : 2;
   const int octets = (a.dst_base % 8 + a.n + 7) / 8, groups = (a.head_dim + kValueDims - 1) / kValueDims;
-  cut.octets = kBlock / kValueDims;  // the block's eight dimensions at once, until the row fills it
+  cut.octets = kBlock / kValueDims;  // the block's dimensions at once, until the row fills it
   while (cut.octets < octets && cut.octets < kBlock) cut.octets *= 2;
   const int rows = kBlock / (a.head_dim / 8) * kKeyPieces;
   cut.key_blocks = a.in_place ? 1 : (a.n + rows - 1) / rows;
   cut.value_blocks = a.in_place ? 1 : (octets + cut.octets - 1) / cut.octets;
   const dim3 grid(cut.key_blocks + groups * cut.value_blocks, a.kv_heads, a.layers);
-  if (a.in_place) hipLaunchKernelGGL((k_kv_gather<true, kDimsInPlace>), grid, dim3(kBlock), 0, s, a, cut);
-  else hipLaunchKernelGGL((k_kv_gather<false, kDimsBetween>), grid, dim3(kBlock), 0, s, a, cut);
+  if (a.in_place) hipLaunchKernelGGL((k_kv_gather<true, kDimsInPlace, 8>), grid, dim3(kBlock), 0, s, a, cut);
+  else if (a.n < kManyRows) hipLaunchKernelGGL((k_kv_gather<false, 4, 2>), grid, dim3(kBlock), 0, s, a, cut);
+  else hipLaunchKernelGGL((k_kv_gather<false, 2, 2>), grid, dim3(kBlock), 0, s, a, cut);
   return hipGetLastError();
 }
 
