@@ -375,14 +375,14 @@ __global__ __launch_bounds__(kWave * WK, 2) void k_attn_tree_direct(TreeAttnArgs
                                                                   float* __restrict__ part_ml) {
   constexpr int kGroups = 8;  // of four dimensions: 32 (g / 4) + 8 (g % 4) + 4 hb .. +3
   constexpr int kStage = 32, kStageSize = kStage * kHeadDim;
-  union Shared {
-    uint16_t stage[WK][2][2][kStageSize];  // K and V, twice
-    struct {
-      v4f o[WK][kGroups][kWave];
-      float m[WK][kTreeCols], l[WK][kTreeCols], out[kTreeCols][kStoreRow];
-    } end;
+  union Wave {
+    uint16_t stage[2][2][kStageSize];  // K and V, twice
+    v4f o[kGroups][kWave];             // in the end
   };
-  __shared__ __attribute__((aligned(16))) Shared sh;
+  __shared__ __attribute__((aligned(16))) Wave sh[WK];
+  __shared__ __attribute__((aligned(16))) float out[kTreeCols][kStoreRow];
+  __shared__ float wave_m[WK][kTreeCols], wave_l[WK][kTreeCols];
+  __shared__ __attribute__((aligned(16))) int odd[WK];
   const int lane = threadIdx.x & (kWave - 1), wk = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int col = lane & 31, hb = lane >> 5;
   const int group = a.heads / a.kv_heads, rows = a.nodes * group;
@@ -411,7 +411,7 @@ __global__ __launch_bounds__(kWave * WK, 2) void k_attn_tree_direct(TreeAttnArgs
 #pragma unroll
     for (int j = 0; j < 4; j++) copy_to_lds(vb + (size_t)(16 * j) * a.vstride + p0, voff, buf[1] + j * 512);
   };
-  if (first < end) copy(first, sh.stage[wk][0]);
+  if (first < end) copy(first, sh[wk].stage[0]);
   TreeTile t;
   t.c = tree_query(query, t.qh, t.ql);
   float mx;
@@ -423,10 +423,10 @@ __global__ __launch_bounds__(kWave * WK, 2) void k_attn_tree_direct(TreeAttnArgs
       const int p0 = st * kStage;
       uint32_t win[1] = {0xffffffffu};
       if (p0 + kStage > a.past) win[0] = tree_sees(a, mask, p0);
-      uint16_t(&buf)[2][kStageSize] = sh.stage[wk][turn];
+      uint16_t(&buf)[2][kStageSize] = sh[wk].stage[turn];
       if (st + WK < end) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the other buffer has been read
-        copy(st + WK, sh.stage[wk][turn ^ 1]);
+        copy(st + WK, sh[wk].stage[turn ^ 1]);
         tree_landed<8>();  // all but those
       } else {
         tree_landed<0>();
@@ -440,15 +440,15 @@ __global__ __launch_bounds__(kWave * WK, 2) void k_attn_tree_direct(TreeAttnArgs
       tree_take(buf[1], t, s, col, hb, p0, a, win);
     }
     t.l = pair_sum(t.l);
-    __syncthreads();  // the stages' LDS is free
+    wave_lds_handoff();  // the stages have been read
 #pragma unroll
     for (int g = 0; g < kGroups; g++) {
       const int dt = g / 4, i = 4 * (g % 4);
-      sh.end.o[wk][g][lane] = v4f{t.o[dt][i], t.o[dt][i + 1], t.o[dt][i + 2], t.o[dt][i + 3]};
+      sh[wk].o[g][lane] = v4f{t.o[dt][i], t.o[dt][i + 1], t.o[dt][i + 2], t.o[dt][i + 3]};
     }
     if (hb == 0) {
-      sh.end.m[wk][col] = t.m;
-      sh.end.l[wk][col] = t.l;
+      wave_m[wk][col] = t.m;
+      wave_l[wk][col] = t.l;
     }
     __syncthreads();
     // Each wave merges its share of the dimensions; the tile's rows leave through LDS.
@@ -456,14 +456,14 @@ __global__ __launch_bounds__(kWave * WK, 2) void k_attn_tree_direct(TreeAttnArgs
     mx = -INFINITY;
 #pragma unroll
     for (int w = 0; w < WK; w++) {
-      wt[w] = sh.end.m[w][col];
+      wt[w] = wave_m[w][col];
       mx = fmaxf(mx, wt[w]);
     }
     t.l = 0.f;
 #pragma unroll
     for (int w = 0; w < WK; w++) {
       wt[w] = wt[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(wt[w] - mx);
-      t.l = fmaf(sh.end.l[w][col], wt[w], t.l);
+      t.l = fmaf(wave_l[w][col], wt[w], t.l);
     }
     const float scale = gridDim.x > 1 ? 1.f : t.l == 0.f ? 0.f : 1.f / t.l;
     float z = 0.f;
@@ -473,7 +473,7 @@ __global__ __launch_bounds__(kWave * WK, 2) void k_attn_tree_direct(TreeAttnArgs
       v4f x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < WK; w++) {
-        const v4f y = sh.end.o[w][g][lane];
+        const v4f y = sh[w].o[g][lane];
 #pragma unroll
         for (int r = 0; r < 4; r++) x[r] = fmaf(y[r], wt[w], x[r]);
       }
@@ -482,10 +482,16 @@ __global__ __launch_bounds__(kWave * WK, 2) void k_attn_tree_direct(TreeAttnArgs
         z = fmaf(x[r], 0.f, z);
         x[r] *= scale;
       }
-      *reinterpret_cast<v4f*>(&sh.end.out[col][32 * (g / 4) + 8 * (g % 4) + 4 * hb]) = x;
+      *reinterpret_cast<v4f*>(&out[col][32 * (g / 4) + 8 * (g % 4) + 4 * hb]) = x;
     }
-    if (!__syncthreads_or(z != 0.f) || care) break;
-    if (first < end) copy(first, sh.stage[wk][0]);
+    const bool mine_odd = __any(z != 0.f);
+    if (lane == 0) odd[wk] = mine_odd;
+    __syncthreads();
+    int some = 0;
+#pragma unroll
+    for (int w = 0; w < WK; w++) some |= odd[w];
+    if (!some || care) break;
+    if (first < end) copy(first, sh[wk].stage[0]);
   }
   const size_t slot = tree_slot(kvh, rows, row0, a.kv_heads, blockIdx.x);
   if (gridDim.x > 1 && wk == 0 && hb == 0 && row0 + col < rows) *reinterpret_cast<f32x2*>(part_ml + 2 * (slot + col)) = f32x2{mx, t.l};
@@ -494,7 +500,7 @@ __global__ __launch_bounds__(kWave * WK, 2) void k_attn_tree_direct(TreeAttnArgs
     if (row0 + r >= rows) break;
     float* dst = gridDim.x > 1 ? part + (slot + r) * kHeadDim
                                : a.out + ((size_t)((row0 + r) / group) * a.heads + kvh * group + (row0 + r) % group) * kHeadDim;
-    *reinterpret_cast<v4f*>(dst + 4 * (i & 15)) = *reinterpret_cast<const v4f*>(&sh.end.out[r][4 * (i & 15)]);
+    *reinterpret_cast<v4f*>(dst + 4 * (i & 15)) = *reinterpret_cast<const v4f*>(&out[r][4 * (i & 15)]);
   }
   if (care) {
     __syncthreads();
