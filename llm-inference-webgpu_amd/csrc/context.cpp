@@ -692,7 +692,7 @@ int qh_attention_tree(qh_ctx* ctx, const float* d_q, const uint16_t* d_key_cache
                ((uintptr_t)d_mask & 7) == 0,
            QH_ERR_INVALID, "q, the caches and out must be 16-byte aligned, the mask 8-byte");
   qh::TreeAttnArgs a{d_q, d_key_cache, d_value_cache, d_mask, d_out, capacity, qh::value_stride(capacity), heads,
-                     kv_heads, past, nodes};
+                     kv_heads, heads / kv_heads, past, nodes};
   OnDevice on(ctx->device);
   QH_HIP(on.err);
   const size_t bytes = qh::attention_tree_floats(nodes, past, heads, kv_heads) * sizeof(float);

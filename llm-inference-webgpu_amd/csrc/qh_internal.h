@@ -249,7 +249,7 @@ struct TreeAttnArgs {
   const uint16_t *kc, *vt;
   const uint64_t* mask;      // [nodes][ceil(nodes / 64)]
   float* out;                // [nodes][heads*64]
-  int capacity, vstride, heads, kv_heads, past, nodes;
+  int capacity, vstride, heads, kv_heads, group, past, nodes;  // group = heads / kv_heads
 };
 // `part` holds attention_tree_floats floats (no initial contents needed).
 hipError_t launch_attention_tree(hipStream_t s, const TreeAttnArgs& a, float* part);

@@ -29,8 +29,13 @@ constexpr int kMaxTreeSplits = 128;
 constexpr float kWeightLog2 = 13.f;  // p is held as 2^13 p of the running maximum's, which is
 constexpr float kMaxSlack = 2.f;     // left behind by up to 2^2: f16 holds up to 2^15
 
-// Where part k of n, even to one, of `count` begins.
-__host__ __device__ inline int tree_part(int count, int k, int n) { return (int)((int64_t)count * k / n); }
+// Parts, even to one: part k of n begins at k * each + min(k, more). The host divides: in the kernels the
+// 64-bit quotients were 250 instructions before a block's first load (63 nodes at 4097 12.75 us for 12.4).
+struct TreeParts {
+  int each, more;
+  __host__ __device__ int at(int k) const { return k * each + (k < more ? k : more); }
+};
+static TreeParts tree_parts(int count, int n) { return {count / n, count % n}; }
 
 __device__ __forceinline__ int tree_key(int r) { return 16 * (r >> 4) + 8 * ((r >> 2) & 1) + 4 * ((r >> 3) & 1) + (r & 3); }
 
@@ -191,7 +196,7 @@ __device__ __forceinline__ void tree_clip(v4u& v, int k0, int total, int from) {
 }
 __device__ __noinline__ void tree_add_odd(TreeAttnArgs a, float* part, int kvh, int row0, int first, int step, int k0, int k1,
                                           int split, int splits) {
-  const int lane = threadIdx.x & (kWave - 1), group = a.heads / a.kv_heads, rows = a.nodes * group;
+  const int lane = threadIdx.x & (kWave - 1), group = a.group, rows = a.nodes * group;
   const uint16_t* vb = a.vt + ((size_t)kvh * kHeadDim + lane) * a.vstride;
   for (int row = row0 + first; row < min(row0 + kTreeCols, rows); row += step) {
     const int node = row / group;
@@ -219,7 +224,7 @@ __device__ __noinline__ void tree_add_odd(TreeAttnArgs a, float* part, int kvh, 
 constexpr int kStoreRow = kHeadDim + 4;  // floats
 __device__ __forceinline__ void tree_store(const TreeAttnArgs& a, float* part, float* part_ml, float* buf, int kvh, int row0,
                                            int split, int splits, int lane, float m, float l, f32x16 (&o)[2]) {
-  const int col = lane & 31, hb = lane >> 5, group = a.heads / a.kv_heads, rows = a.nodes * group;
+  const int col = lane & 31, hb = lane >> 5, group = a.group, rows = a.nodes * group;
   const float scale = splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
   for (int g = 0; g < 8; g++) {
@@ -368,10 +373,11 @@ __device__ __forceinline__ void tree_take(const uint16_t* vbuf, TreeTile& t, f32
 // 32-key stages w, w + WK, ... of it in two buffers of its own, the next one on its way, with no barrier. The waves'
 // states merge through LDS, each wave merging its share of the dimensions over all of them in order.
 // Bound: latency (a launch, q and a stage from memory, the joining of the waves). 14 heads of 2 kv heads: 5 nodes at
-// 123 (4 stages, one launch) 6.0 us; 16 at 1024 6.9 and 63 at 4097 10.3, and 3.3 and 3.6 for the merge. (Operands
-// straight from the caches instead of through LDS: 12.7 for 11.1 at 16 nodes, both launches of an earlier form.)
+// 123 (4 stages, one launch) 5.7 us; 16 at 1024 6.7 and 63 at 4097 9.9, and 3.3 and 3.5 for the merge. Of the 6.7 a
+// block has q after 1.5, its stage after another 0.4, does it in 0.8 and joins its waves in 1. (Operands straight
+// from the caches instead of through LDS: 12.7 for 11.1 at 16 nodes, both launches of an earlier form.)
 template <int WK>
-__global__ __launch_bounds__(kWave * WK, 2) void k_attn_tree_direct(TreeAttnArgs a, float* __restrict__ part,
+__global__ __launch_bounds__(kWave * WK, 2) void k_attn_tree_direct(TreeAttnArgs a, TreeParts parts, float* __restrict__ part,
                                                                   float* __restrict__ part_ml) {
   constexpr int kGroups = 8;  // of four dimensions: 32 (g / 4) + 8 (g % 4) + 4 hb .. +3
   constexpr int kStage = 32, kStageSize = kStage * kHeadDim;
@@ -385,14 +391,13 @@ __global__ __launch_bounds__(kWave * WK, 2) void k_attn_tree_direct(TreeAttnArgs
   __shared__ __attribute__((aligned(16))) int odd[WK];
   const int lane = threadIdx.x & (kWave - 1), wk = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int col = lane & 31, hb = lane >> 5;
-  const int group = a.heads / a.kv_heads, rows = a.nodes * group;
+  const int group = a.group, rows = a.nodes * group;
   const int kvh = blockIdx.z, total = a.past + a.nodes;
   const int row0 = blockIdx.y * kTreeCols, row = min(row0 + col, rows - 1);  // past the end, a copy of the last
   const int node = row / group;
   const size_t at = (size_t)node * a.heads + kvh * group + row % group;
   const uint64_t* mask = a.mask + (size_t)node * ((a.nodes + 63) / 64);
-  const int stages = (total + kStage - 1) / kStage;
-  const int begin = tree_part(stages, blockIdx.x, gridDim.x), end = tree_part(stages, blockIdx.x + 1, gridDim.x);
+  const int begin = parts.at(blockIdx.x), end = parts.at(blockIdx.x + 1);  // 32-key stages
   const int first = begin + wk;
 
   TreeQuery query;
@@ -563,7 +568,7 @@ __device__ __forceinline__ void tree_step(const uint16_t* kbuf, const uint16_t* 
   }
 }
 
-__global__ __launch_bounds__(kWave * kTreeWaves, 2) void k_attn_tree_staged(TreeAttnArgs a, int splits, int tiles,
+__global__ __launch_bounds__(kWave * kTreeWaves, 2) void k_attn_tree_staged(TreeAttnArgs a, TreeParts parts, int splits, int tiles,
                                                                           float* __restrict__ part, float* __restrict__ part_ml) {
   __shared__ __attribute__((aligned(16))) uint16_t kbuf[2][kTreeStage * kHeadDim], vbuf[2][kTreeStage * kHeadDim];
   __shared__ __attribute__((aligned(16))) float out_buf[kTreeWaves][kTreeCols * kStoreRow];
@@ -574,19 +579,18 @@ __global__ __launch_bounds__(kWave * kTreeWaves, 2) void k_attn_tree_staged(Tree
   const int ranges = splits * a.kv_heads, b = blockIdx.x;
   const int range = ranges % 8 ? b % ranges : (b & 7) + 8 * ((b >> 3) / tiles);
   const int split = range % splits, kvh = range / splits;
-  const int group = a.heads / a.kv_heads, rows = a.nodes * group;
+  const int group = a.group, rows = a.nodes * group;
   const int total = a.past + a.nodes;
   const int tile = (ranges % 8 ? b / ranges : (b >> 3) % tiles) * waves + wave;
   const int row = min(tile * kTreeCols + col, rows - 1);  // past the end, a copy of the last
   const int node = row / group, head = kvh * group + row % group;
   const uint64_t* mask = a.mask + (size_t)node * ((a.nodes + 63) / 64);
-  const int stages = (total + kTreeStage - 1) / kTreeStage;
   // Stages with nodes in them, which are hidden and taken one by one, take twice the time of those before and count
   // twice where the ranges are cut: 512 nodes at 32768 134 us, where they counted once 143; 256 nodes 75 and 76. Where
-  // there are ranges, each has six stages or more (tree_plan), so none is left without.
+  // there are ranges, each counts six or more (tree_plan), so none is left without a stage.
   const int before = a.past / kTreeStage;
   auto cut = [&](int k) {
-    const int v = tree_part(2 * stages - before, k, splits);
+    const int v = parts.at(k);
     return v <= before ? v : before + (v - before) / 2;
   };
   const int first = cut(split), end = cut(split + 1);
@@ -681,7 +685,7 @@ __global__ __launch_bounds__(kWave * kTreeWaves, 2) void k_attn_tree_staged(Tree
 template <int kFlight>
 __global__ __launch_bounds__(kBlock) void k_attn_tree_merge(TreeAttnArgs a, const float* __restrict__ part,
                                                             const float* __restrict__ part_ml, int splits) {
-  const int lane = threadIdx.x & (kWave - 1), group = a.heads / a.kv_heads, rows = a.nodes * group;
+  const int lane = threadIdx.x & (kWave - 1), group = a.group, rows = a.nodes * group;
   const int at = blockIdx.x * (kBlock / kWave) + threadIdx.x / kWave;
   if (at >= rows * a.kv_heads) return;
   const int kvh = at / rows, row = at % rows, k = lane >> 4, d = lane & 15;
@@ -786,10 +790,13 @@ size_t attention_tree_floats(int nodes, int past, int heads, int kv_heads) {
 hipError_t launch_attention_tree(hipStream_t s, const TreeAttnArgs& a, float* part) {
   const TreePlan t = tree_plan(a.nodes, a.past, a.heads, a.kv_heads);
   float* ml = part + (size_t)a.nodes * a.heads * t.splits * kHeadDim;
+  const int total = a.past + a.nodes;
   if (t.direct)
-    hipLaunchKernelGGL((k_attn_tree_direct<8>), dim3(t.splits, t.tiles, a.kv_heads), dim3(8 * kWave), 0, s, a, part, ml);
+    hipLaunchKernelGGL((k_attn_tree_direct<8>), dim3(t.splits, t.tiles, a.kv_heads), dim3(8 * kWave), 0, s, a,
+                       tree_parts((total + 31) / 32, t.splits), part, ml);
   else
-    hipLaunchKernelGGL(k_attn_tree_staged, dim3(t.splits * a.kv_heads * t.tiles), dim3(t.waves * kWave), 0, s, a, t.splits,
+    hipLaunchKernelGGL(k_attn_tree_staged, dim3(t.splits * a.kv_heads * t.tiles), dim3(t.waves * kWave), 0, s, a,
+                       tree_parts(2 * ((total + kTreeStage - 1) / kTreeStage) - a.past / kTreeStage, t.splits), t.splits,
                        t.tiles, part, ml);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || t.splits == 1) return e;
