@@ -183,6 +183,24 @@ def test_attention_of_a_chain_is_causal_attention(ctx):
     assert np.linalg.norm(got - want) <= 2e-6 * np.linalg.norm(want)  # two f32 evaluations, 1e-6 each
 
 
+@pytest.mark.parametrize("nodes,past,heads,kv", [(3, 20, 14, 2), (17, 1500, 9, 3), (64, 12900, 32, 1)])
+def test_attention_writes_its_rows_alone(ctx, nodes, past, heads, kv):
+    """What lies before and behind out, the queries, the mask and the caches keep their bits."""
+    rng = np.random.default_rng(nodes)
+    keys, values = _caches(rng, kv, past + nodes + 5, past + nodes)
+    q = rng.standard_normal((nodes, heads * 64)).astype(np.float32)
+    mask = T.pack(T.plan(T.random_tree(rng, nodes))[1])
+    room = np.full(q.size + 128, 7.25, np.float32)
+    given = (q, keys, values, mask)
+    bufs, out = [ctx.upload(x) for x in given], ctx.upload(room)
+    inner = type(out)(ctx, out.ptr + 256, q.nbytes)
+    ctx.attention_tree(bufs[0], bufs[1], bufs[2], past + nodes + 5, bufs[3], inner, nodes, past, heads, kv)
+    got = out.read()
+    assert (got[:64] == 7.25).all() and (got[-64:] == 7.25).all() and (got[64:-64] != 7.25).all()
+    for b, x in zip(bufs, given):
+        np.testing.assert_array_equal(b.read(np.uint8), np.frombuffer(np.ascontiguousarray(x).tobytes(), np.uint8))
+
+
 def test_attention_behind_four_billion_bytes(ctx):
     """A cache whose last kv head starts behind 2^32 bytes and 2^31 values."""
     rng = np.random.default_rng(6)
