@@ -25,7 +25,7 @@ namespace qh {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int kTreeCols = 32;    // rows of a wave's tile
-constexpr int kMaxTreeSplits = 128;
+constexpr int kMaxTreeSplits = 128;  // of the staged kernel
 constexpr float kWeightLog2 = 13.f;  // p is held as 2^13 p of the running maximum's, which is
 constexpr float kMaxSlack = 2.f;     // left behind by up to 2^2: f16 holds up to 2^15
 
@@ -373,7 +373,7 @@ __device__ __forceinline__ void tree_take(const uint16_t* vbuf, TreeTile& t, f32
 // 32-key stages w, w + WK, ... of it in two buffers of its own, the next one on its way, with no barrier. The waves'
 // states merge through LDS, each wave merging its share of the dimensions over all of them in order.
 // Bound: latency (a launch, q and a stage from memory, the joining of the waves). 14 heads of 2 kv heads: 5 nodes at
-// 123 (4 stages, one launch) 5.7 us; 16 at 1024 6.7 and 63 at 4097 9.9, and 3.3 and 3.5 for the merge. Of the 6.7 a
+// 123 (4 stages, one launch) 5.7 us; 16 at 1024 6.5 and 63 at 4097 9.8, and 3.1 and 3.2 for the merge. Of the 6.5 a
 // block has q after 1.5, its stage after another 0.4, does it in 0.8 and joins its waves in 1. (Operands straight
 // from the caches instead of through LDS: 12.7 for 11.1 at 16 nodes, both launches of an earlier form.)
 template <int WK>
@@ -680,7 +680,7 @@ __global__ __launch_bounds__(kWave * kTreeWaves, 2) void k_attn_tree_staged(Tree
 // k, k + 4, ..., and the four sums are added in order: o = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s.
 // kFlight of a lane's splits are loaded at once, the first ones before the maximum is known: 1 up to 4 splits, 4 up to 16, 8
 // beyond (64 of 14 rows: 12.2 us with 8 and 15.2 with 4, the attention included; 2 of 3584: 24.9 and 24.0).
-// Bound: latency of a load behind a launch; bytes for many rows (14 MB for 896 rows of 60 ranges).
+// Bound: latency of a load behind a launch, 3.1 us; bytes for many rows (14 MB for 896 rows of 60 ranges).
 // Joined by the last block of a tile instead, the states would cross the XCDs through fences that take as long.
 template <int kFlight>
 __global__ __launch_bounds__(kBlock) void k_attn_tree_merge(TreeAttnArgs a, const float* __restrict__ part,
@@ -756,13 +756,25 @@ TreePlan tree_plan(int nodes, int past, int heads, int kv_heads) {
   if (t.direct) {
     t.waves = kTreeWaves;
     t.tiles = cols;
-    // In us: a step takes its block 0.15, a merge 2.4, 0.045 a range and 0.5 per 1000 rows. So sqrt(3.3 steps) ranges, as
-    // the CUs allow, or one without a merge. Measured with 1 / 4 / 8 / 16 / 32 / 64: 5 nodes at 512 8.4 / 9.0 / 9.1 / 9.4,
-    // at 1040 10.9 / 10.1 / 10.0 / 9.2 / 9.6, at 4097 25.5 / 13.8 / 11.3 / 10.4 / 10.3 / 11.0, one at 32768 8 to 128: 27.3 /
-    // 18.2 / 13.3 / 12.2 / 14.1; 200 nodes at 1024, 16 heads of one kv head, with 1 / 2: 11.7 / 13.3.
+    // As many ranges as a round of the merge's loads takes, at most one block to a CU, in fours. In us: a step takes its
+    // block 0.15, the merge 2.6, 0.5 per 1000 rows and kMore. Measured with 1 / 8 / 16 / 32 / 64 / 128: 5
+    // nodes at 600 8.1 / 8.9 / 8.9, at 1024 10.3 / 8.8 / 8.5 / 9.1, one at 4096 23.8 / 9.6 / 8.4 / 7.9 / 9.0 / 11.5, at 32768
+    // 157 / 26.7 / 17.3 / 12.6 / 11.6 / 13.7, with 36 13.7; 16 at 1024 with 8 / 12 / 16 9.5 / 8.9 / 9.2. 200 nodes at 1024, 16 heads of one kv head, 1 / 2: 11.7 / 13.3. Ranges
+    // in fours: 63 nodes at 4097 with 8 / 9 12.0 / 12.7, 20 at 32768 with 24 / 25 16.6 / 20.5 (blocks of a range on an XCD
+    // or two); 40 at 4096 with 12 / 14 11.0 / 11.3, at 16384 17.0 / 16.8.
     const int room = 256 / std::min(256, t.tiles * kv_heads);
-    t.splits = std::min(std::min(room, kMaxTreeSplits), (int)(sqrt(3.3 * steps) + 0.5));
-    if (0.15 * steps <= 0.15 * steps / t.splits + 2.4 + 0.045 * t.splits + 0.0005 * nodes * heads) t.splits = 1;
+    constexpr int kRanges[] = {8, 12, 16, 32, 64, 96, 128};
+    constexpr double kMore[] = {0.25, 0.35, 0.5, 0.95, 2.4, 4.2, 5.6};
+    double least = 0.15 * steps - 2.6 - 0.0005 * nodes * heads;
+    t.splits = 1;
+    for (int i = 0; i < 7; i++) {
+      int n = std::min(std::min(room, steps), kRanges[i]);
+      if (n > 8) n &= ~3;
+      const double cost = 0.15 * steps / n + kMore[i];
+      if (cost >= least) continue;
+      least = cost;
+      t.splits = n;
+    }
     return t;
   }
   const int stages = (total + kTreeStage - 1) / kTreeStage;
