@@ -41,7 +41,7 @@ __device__ __forceinline__ double fma_const(double a, double b, double c) {  // 
   return r;
 }
 
-// 2^x for x <= 0 (NaN: 0): 2^rint(x) times 1 + f g(f), f the rest in [-1/2, 1/2] and g the polynomial
+// 2^x for x <= 1/2 (NaN: 0): 2^rint(x) times 1 + f g(f), f the rest in [-1/2, 1/2] and g the polynomial
 // through (2^f - 1) / f at eleven Chebyshev points (8e-18 off): 11 multiply-adds.
 __device__ __forceinline__ double exp2_f64(double x) {
   x = fmax(x, -1100.0);  // 2^-1100 is 0; so is NaN's
@@ -61,11 +61,38 @@ __device__ __forceinline__ double exp2_f64(double x) {
   return __builtin_ldexp(p, (int)n);
 }
 
-// e of a logit l <= m, 0 for NaN; k = log2(e) / T. FINITE: m is.
-template <bool FINITE = false>
-__device__ __forceinline__ double token_weight(float l, float m, double k) {
-  if constexpr (FINITE) return exp2_f64(((double)l - (double)m) * k);
-  return exp2_f64(l == m ? 0.0 : ((double)l - (double)m) * k);  // equal infinities weigh 1
+// What the weights of a row, a chunk or a wave with the maximum m are relative to, k = log2(e) / T: e = 2^(k l - E) with
+// the whole number E = rint(k m), so that sums of different maxima differ by a power of two; or, where k m is not
+// below 2^30 in size (NaN and infinities too), e = 2^(k (l - m)), equal infinities weighing 1.
+struct VerifyRef {
+  double e;
+  float m;
+  bool whole;
+};
+__device__ __forceinline__ VerifyRef verify_ref(float m, double k) {
+  const double e = __builtin_rint((double)m * k);
+  return {e, m, fabs(e) < 0x1p30};
+}
+// e of a logit l <= m, 0 for NaN.
+__device__ __forceinline__ double whole_weight(float l, const VerifyRef& r, double k) { return exp2_f64(fma((double)l, k, -r.e)); }
+__device__ __forceinline__ double other_weight(float l, const VerifyRef& r, double k) {
+  return exp2_f64(l == r.m ? 0.0 : ((double)l - (double)r.m) * k);
+}
+__device__ __forceinline__ double token_weight(float l, const VerifyRef& r, double k) {  // any lane its r
+  double w = whole_weight(l, r, k);
+  if (__any(!r.whole)) w = r.whole ? w : other_weight(l, r, k);
+  return w;
+}
+// A sum relative to `from` as one relative to `to`, from.m <= to.m.
+__device__ __forceinline__ double verify_shift(double sum, const VerifyRef& from, const VerifyRef& to, double k) {
+  double s = __builtin_ldexp(sum, (int)(from.e - to.e));
+  const bool other = sum != 0.0 && !(from.whole && to.whole);
+  if (__any(other)) {
+    const double w = from.whole ? exp2_f64(fma(-(double)to.m, k, from.e))
+                     : to.whole ? whole_weight(from.m, to, k) : other_weight(from.m, to, k);
+    s = other ? sum * w : s;
+  }
+  return s;
 }
 
 // The maximum over a wave, NaN ignored; every lane gets it.
@@ -194,6 +221,7 @@ __global__ __launch_bounds__(kRowsThreads) void k_verify_rows(VerifyArgs a, Veri
     if (lane == 0) wb[wave] = best;
   } else {
     const double k2 = 1.44269504088896340736 / a.temperature;
+    const VerifyRef ref = verify_ref(m, k2);
     double s = 0.0;
     if (fabsf(m) < INFINITY) {
       if (__any(hide)) {
@@ -202,10 +230,15 @@ __global__ __launch_bounds__(kRowsThreads) void k_verify_rows(VerifyArgs a, Veri
 #pragma unroll
           for (int k = 0; k < 4; k++) x[g][k] = hide >> (4 * g + k) & 1 ? -INFINITY : x[g][k];
       }
+      if (ref.whole) {
 #pragma unroll
-      for (int g = 0; g < G; g++)
+        for (int g = 0; g < G; g++)
 #pragma unroll
-        for (int k = 0; k < 4; k++) s += token_weight<true>(x[g][k], m, k2);
+          for (int k = 0; k < 4; k++) s += whole_weight(x[g][k], ref, k2);
+      } else {
+        for (int g = 0; g < G; g++)
+          for (int k = 0; k < 4; k++) s += other_weight(x[g][k], ref, k2);
+      }
     } else {  // equal infinities, or nothing but NaN
 #pragma unroll
       for (int g = 0; g < G; g++)
@@ -230,7 +263,8 @@ __global__ __launch_bounds__(kRowsThreads) void k_verify_rows(VerifyArgs a, Veri
       if (wm[w] == top) best = min(best, wb[w]);
     if (tid == 0) *out = {0.0, top, best};
   } else {
-    double s = ws[tid] * token_weight(wm[tid], top, 1.44269504088896340736 / a.temperature);
+    const double k2 = 1.44269504088896340736 / a.temperature;
+    double s = verify_shift(ws[tid], verify_ref(wm[tid], k2), verify_ref(top, k2), k2);
 #pragma unroll
     for (int off = 1; off < W; off <<= 1) s += __shfl_xor(s, off);
     if (tid == 0) *out = {s, top, 0};
@@ -261,10 +295,11 @@ __device__ __forceinline__ void verify_row(const VerifyPart* part, const VerifyP
   for (int r = 0; r < N; r++) m[r] = verify_max(m[r]);
 #pragma unroll
   for (int r = 0; r < N; r++) {
-    s[r] = p[r].sum * token_weight(p[r].max, m[r], k2);
+    const VerifyRef to = verify_ref(m[r], k2);
+    s[r] = verify_shift(p[r].sum, verify_ref(p[r].max, k2), to, k2);
     for (int c = lane + kWave; c < chunks && r < rows; c += kWave) {
       const VerifyPart q = part[(size_t)r * chunks + c];
-      s[r] = fma(q.sum, token_weight(q.max, m[r], k2), s[r]);
+      s[r] += verify_shift(q.sum, verify_ref(q.max, k2), to, k2);
     }
   }
 #pragma unroll
@@ -345,26 +380,25 @@ __global__ __launch_bounds__(kRowsThreads) void k_verify_residual(VerifyArgs a, 
   double sum1[1];
   verify_row<1>(part + (size_t)node * chunks, p, 1, chunks, k2, max1, sum1);
   const float m = max1[0];
+  const VerifyRef ref = verify_ref(m, k2);
   const double inv_z = 1.0 / sum1[0];
   VerifyTest t = {0.0, 1.0};
 #pragma unroll
   for (int r = 0; r < kResiduals; r++) {
     if (r > round) break;
-    if (verify_accept(t, token_weight(child[r].logit, m, k2), inv_z, child[r].prob, u[r])) return;
+    if (verify_accept(t, token_weight(child[r].logit, ref, k2), inv_z, child[r].prob, u[r])) return;
     t.a += t.f;
     if (r < round) verify_reject(t, team_sum<64>(sums[r]));
   }
   double s = 0.0;
-  if (fabsf(m) < INFINITY) {
+  if (ref.whole) {
 #pragma unroll
     for (int g = 0; g < G; g++)
 #pragma unroll
-      for (int k = 0; k < 4; k++) s += residual_weight(token_weight<true>(x[g][k], m, k2), inv_z, t.a, q[g][k]);
+      for (int k = 0; k < 4; k++) s += residual_weight(whole_weight(x[g][k], ref, k2), inv_z, t.a, q[g][k]);
   } else {
-#pragma unroll
     for (int g = 0; g < G; g++)
-#pragma unroll
-      for (int k = 0; k < 4; k++) s += residual_weight(x[g][k] == m ? 1.0 : 0.0, inv_z, t.a, q[g][k]);
+      for (int k = 0; k < 4; k++) s += residual_weight(other_weight(x[g][k], ref, k2), inv_z, t.a, q[g][k]);
   }
   s = team_sum<64>(s);
   if (lane == 0) ws[wave] = s;
@@ -434,7 +468,7 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(VerifyArgs a, cons
     }
   }
   __syncthreads();
-  if (up >= 0) weight[tid] = token_weight(own.logit, row_max[up], k2);
+  if (up >= 0) weight[tid] = token_weight(own.logit, verify_ref(row_max[up], k2), k2);
   __syncthreads();
 
   int at = 0, count = 1;
@@ -447,11 +481,12 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(VerifyArgs a, cons
   auto make_sums = [&]() {
     const float* row = a.logits + (size_t)at * a.vocab;
     const float* draft = t.a == 0.0 ? nullptr : a.draft + (size_t)at * a.vocab;
+    const VerifyRef ref = verify_ref(row_max[at], k2);
     __syncthreads();
     for (int c = wave; c < chunks; c += W) {
       double s = 0.0;
       for (int i = c * kChunkV + lane; i < min(a.vocab, (c + 1) * kChunkV); i += kWave) {
-        const double e = token_weight(row[i], row_max[at], k2);
+        const double e = token_weight(row[i], ref, k2);
         s += draft ? residual_weight(e, inv_z, t.a, draft[i]) : e;
       }
       s = team_sum<64>(s);
@@ -568,7 +603,7 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(VerifyArgs a, cons
   // The weights that are left at the last node: the residual's, or e, without the children's tokens
   // where they are points (all of them again if nothing else is left).
   const VerifyPart* pa = part + (size_t)at * chunks;
-  const float m = row_max[at];
+  const VerifyRef ref = verify_ref(row_max[at], k2);
   const bool plain = point || t.a == 0.0;
   const bool without = point && kids && row_sum[at] != 0.0;
   const double* last = !plain && tested <= rounds ? res + ((size_t)(tested - 1) * a.nodes + at) * chunks : nullptr;
@@ -595,14 +630,14 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(VerifyArgs a, cons
       }
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-      w[k] = token_weight(x[0][k], m, k2);
+      w[k] = token_weight(x[0][k], ref, k2);
       if (!plain) w[k] = residual_weight(w[k], inv_z, t.a, q[0][k]);
       if (hide >> k & 1) w[k] = 0.0;
     }
   };
   if (no_sums && plain) make_sums();  // a residual's are there from the last rejection
   auto chunk_sum = [&](int c) -> double {
-    return c >= chunks ? 0.0 : no_sums ? sums[c] : plain ? pa[c].sum * token_weight(pa[c].max, m, k2) : last[c];
+    return c >= chunks ? 0.0 : no_sums ? sums[c] : plain ? verify_shift(pa[c].sum, verify_ref(pa[c].max, k2), ref, k2) : last[c];
   };
   // The first chunk whose running sum passes the target (every wave for itself, 64 chunks at a time);
   // where the rounding of the total leaves none, the last one with a weight.

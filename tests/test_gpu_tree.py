@@ -385,6 +385,23 @@ def test_verify_tree_with_nothing_left(ctx):
     assert _verify(ctx, logits, draft, tokens, parent, 1.0, u) == T.verify(logits, draft, tokens, parent, 1.0, u) == ([0], 7)
 
 
+@pytest.mark.parametrize("how", ["lookup", "sampled"])
+@pytest.mark.parametrize("temperature", [1e-30, 1e-9, 1e-3, 1e3, 1e30])
+def test_verify_tree_of_any_scale(ctx, how, temperature):
+    """Logits from the temperature's size to 2^30 and more times it, some masked by the lowest f32, chunks of those alone."""
+    vocab, nodes = 9000, 9
+    for seed, scale in enumerate((1.0, 30.0, 1e4, 2.0**29, 2.0**31, 1e12)):
+        rng = np.random.default_rng(seed)
+        logits, q, tokens, parent, u = _drafts(rng, nodes, vocab, how)
+        top = min(temperature * scale, 1e37)
+        logits = np.clip(logits * np.float64(temperature) - top * rng.integers(0, 2, (nodes, 1)), -3e38, 3e38).astype(np.float32)
+        logits[rng.random(logits.shape) < 0.3] = np.finfo(np.float32).min
+        logits[seed % nodes, 4096:8192] = np.finfo(np.float32).min
+        for i in range(1, nodes, 2):
+            tokens[i] = logits[parent[i]].argmax()
+        assert _verify(ctx, logits, q, tokens, parent, temperature, u) == T.verify(logits, q, tokens, parent, temperature, u), scale
+
+
 @pytest.mark.parametrize("how", ["greedy", "lookup", "sampled"])
 @pytest.mark.parametrize("nodes,vocab", [(14, 9001), (64, 4100), (200, 9000)])
 def test_verify_tree_of_one_generation(ctx, how, nodes, vocab):
