@@ -421,7 +421,8 @@ __device__ __forceinline__ double lane_value(double v, int lane) {
 // Bound: latency (three rounds of loads, one after another, and the f64 arithmetic between them): 9.5 us for 64 looked
 // up nodes of 151936 and for 32 sampled ones. (A walk node by node over LDS took 25000 of the kernel's 45000 cycles: 33.8
 // us for both launches of 64 nodes, 22.6 with a node's children tested all at once in the lanes of a wave. All of 32
-// nodes' F summed before the walk instead of the few it asks for: 11.9.)
+// nodes' F summed before the walk instead of the few it asks for: 11.9. The drawn token found in a quarter of its chunk, from
+// sums of quarters: 9.3, but both launches 22.7 for 21.6.)
 __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(VerifyArgs a, const VerifyPart* __restrict__ part,
                                                               const VerifyKid* __restrict__ kid,
                                                               const double* __restrict__ res, int rounds, int chunks) {
