@@ -611,6 +611,12 @@ struct TreeScratch {
       for (const qh_ctx::TreePiece& p : ctx->tree_pieces)
         if (p.capture == id && p.bytes >= bytes) ptr = p.ptr;
       if (ptr) return;
+      try {
+        ctx->tree_pieces.reserve(ctx->tree_pieces.size() + 1);
+      } catch (...) {  // not through a C entry
+        err = hipErrorOutOfMemory;
+        return;
+      }
       hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;  // allocations are allowed
       err = hipThreadExchangeStreamCaptureMode(&mode);
       if (err != hipSuccess) return;
